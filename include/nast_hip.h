@@ -179,6 +179,49 @@ int nast_softmax_bwd_f32(const float* gy, nast_rows gyr, const float* y, nast_ro
 int nast_first_eos_length_i64(const int64_t* tokens, int64_t* lengths, int B, int L, int64_t eos, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * A teacher's top logits, distillation from them, verification of drafted tokens.  No counterpart in the reference.
+ * Rows of logits in fp32, bf16 or fp16 (`dtype`); all arithmetic in fp32 or double.  `temp` > 0 divides the logits.
+ * Sizes: V < 2^24, lists of 1..256 slots, rows * (chunks of a row) < 2^24.  Workspaces are the caller's (sizes below; 256-byte
+ * aligned; 0 bytes: may be NULL), hold nothing between calls and must not be shared by calls that may overlap.
+ * ---------------------------------------------------------------------------------------------- */
+#define NAST_F32 0
+#define NAST_BF16 1
+#define NAST_F16 2
+
+/* The k largest logits of every row, largest first, ties to the lower id, NaN above everything: values [rows, k] in the logits'
+ * type, index int64 [rows, k], and lse[r] = log sum_v exp(x[r, v] / temp) (NaN where the row holds a NaN or +inf). */
+int64_t nast_top_logits_workspace_bytes(int rows, int V, int k, int dtype);
+int nast_top_logits(const void* x, int dtype, nast_rows xr, void* values, int64_t* index, float* lse, int rows, int V, int k,
+                    double temp, void* workspace, void* stream);
+
+/* Loss of a student's rows z [rows, V] against a teacher's lists: t [rows, K] the teacher's logits (`t_dtype`), idx int64 [rows, K]
+ * their ids.  A slot whose id lies outside [0, V) or whose logit is -inf is unused; an id in two slots counts in both.
+ *   p_j = exp(t_j / temp - c_r),  q = softmax(z_r / temp)
+ *   loss[r] = sum_j p_j (log p_j - log q[id_j])                         c_r = logsumexp of the used t_j / temp     (lse_t NULL)
+ *           + p_rest (log p_rest - log q_rest)                          c_r = lse_t[r]                             (lse_t given)
+ * p_rest = max(0, 1 - sum p_j), q_rest the student's probability of every token in no used slot (the term is left out where the
+ * student has none).  A row without a used slot: loss 0, gradient 0.  stats: 6 doubles per row for the backward pass. */
+int64_t nast_top_distill_workspace_bytes(int rows, int V, int dtype);
+int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, const void* t, int t_dtype, const int64_t* idx, int K,
+                         const float* lse_t, float* loss, double* stats, int rows, int V, double temp, void* workspace, void* stream);
+/* gx[r, v] = g[r] * d loss[r] / d x[r, v], in the logits' type; gx must not be x.  Rows with g = 0 are zeros whatever x holds. */
+int nast_top_distill_bwd(const float* g, const void* x, int dtype, nast_rows xr, const void* t, int t_dtype, const int64_t* idx,
+                         int K, const double* stats, void* gx, nast_rows gxr, int rows, int V, double temp, void* stream);
+
+/* Speculative sampling.  target [B, N+1, V], draft [B, N, V] or NULL (logits; batch and row strides in elements, the last axis
+ * contiguous), tokens int64 [B, N] the drafts, lengths int64 [B] how many of them count (clamped to 0..N; NULL: N), u [B, N]
+ * uniforms, E [B, V] Exp(1) draws (all contiguous).  With p_i, q_i the softmax of target / draft row i over temp (draft NULL: q_i is one at d_i):
+ *   d_i stands while q_i(d_i) > 0 and u_i q_i(d_i) < p_i(d_i);  accepted[b] = how many stand in a row from the first;
+ *   out[b] = the accepted drafts, then argmax_v w_v / E_v (ties to the lower id), then -1;
+ *   w = (p_i - q_i)+ at the refused place i (p_i where that is zero everywhere), p_n behind the last draft.
+ * A row that holds a NaN or +inf or nothing but -inf has no distribution: a draft is refused at a target row or draft row of that
+ * kind, q is then taken as 0, and the token drawn from such a target row is -1.  A drafted id outside [0, V) is refused. */
+int64_t nast_verify_draft_workspace_bytes(int B, int N, int V, int dtype);
+int nast_verify_draft(const void* target, int64_t target_bs, int64_t target_rs, const void* draft, int64_t draft_bs,
+                      int64_t draft_rs, int dtype, const int64_t* tokens, const float* u, const float* E, const int64_t* lengths,
+                      int64_t* out, int64_t* accepted, int B, int N, int V, double temp, void* workspace, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Embedding assembly: out[b, e + i, :] = tok(b, i) + pos[i],  out[b, 0..e-1, :] = extra rows.
  * Replaces: torch.cat((style_emb, embed(tokens, pos)), 1) -- transformer.py:63-65, :141-148, :225-231.
  *   tok(b,i) = tok_weight[ids[b,i]]  (ids != NULL)   or   tok_rows[b*L + i]  (soft tokens: GEMM output).

@@ -81,6 +81,13 @@ SIGNATURES = {
     "nast_nll_log_softmax_bwd_f32": [c_fp, c_fp, Rows, c_fp, c_fp, Rows, _i, _i, _f, c_fp],
     "nast_lse_nll_f32": [c_fp, Rows, c_fp, c_fp, c_fp, _i, _i, _f, c_fp],
     "nast_nll_logits_bwd_f32": [c_fp, c_fp, Rows, c_fp, c_fp, c_fp, Rows, _i, _i, _f, c_fp],
+    "nast_top_logits_workspace_bytes": [_i] * 4,
+    "nast_top_logits": [c_fp, _i, Rows, c_fp, c_fp, c_fp, _i, _i, _i, _d, c_fp, c_fp],
+    "nast_top_distill_workspace_bytes": [_i] * 3,
+    "nast_top_distill_fwd": [c_fp, _i, Rows, c_fp, _i, c_fp, _i, c_fp, c_fp, c_fp, _i, _i, _d, c_fp, c_fp],
+    "nast_top_distill_bwd": [c_fp, c_fp, _i, Rows, c_fp, _i, c_fp, _i, c_fp, c_fp, Rows, _i, _i, _d, c_fp],
+    "nast_verify_draft_workspace_bytes": [_i] * 4,
+    "nast_verify_draft": [c_fp, _i64, _i64, c_fp, _i64, _i64, _i] + [c_fp] * 6 + [_i] * 3 + [_d, c_fp, c_fp],
     "nast_lp_logits_fwd_f32": [c_fp] * 5 + [_i] * 4 + [c_fp],
     "nast_lp_logits_bwd_f32": [c_fp] * 8 + [_i] * 4 + [c_fp],
     "nast_lp_decode_workspace_bytes": [_i] * 6,
@@ -93,7 +100,9 @@ SIGNATURES = {
     "nast_prof_end": [C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(C.c_int64)],
     "nast_prof_get": [_i, C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(C.c_int64)],
 }
-_RESTYPES = {"nast_last_error": C.c_char_p, "nast_lp_decode_workspace_bytes": C.c_int64}
+_RESTYPES = {"nast_last_error": C.c_char_p, "nast_lp_decode_workspace_bytes": C.c_int64,
+             "nast_top_logits_workspace_bytes": C.c_int64, "nast_top_distill_workspace_bytes": C.c_int64,
+             "nast_verify_draft_workspace_bytes": C.c_int64}
 
 _lib = None
 

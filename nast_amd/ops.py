@@ -4,16 +4,18 @@ PyTorch is used here for device memory (torch.empty), the current HIP stream and
 every numeric operation is a hand-written gfx950 kernel reached through the C-ABI (nast_amd/_lib.py).
 There is no CPU / eager fallback: a non-CUDA tensor raises.
 """
+import collections
 import ctypes as C
 import math
 import os
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 import contextlib
 
-from ._lib import GemmDesc, Rows, GEMM_RELU, GEMM_ATOMIC, GEMM_ACCUM, GEMM_BF16, call
+from ._lib import GemmDesc, Rows, GEMM_RELU, GEMM_ATOMIC, GEMM_ACCUM, GEMM_BF16, call, load
 
 F32 = torch.float32
 
@@ -1120,6 +1122,223 @@ class GumbelSoftmaxFn(torch.autograd.Function):
 def gumbel_softmax_sample(logits, E=None, mask=None, tau=1.0, noise_off=False):
     """-> (y_soft, argmax index)"""
     return GumbelSoftmaxFn.apply(logits, E, mask, float(tau), noise_off)
+
+
+# ------------------------------------------------------------------------------------------------
+# a teacher's top logits, distillation from them, verification of drafted tokens
+# ------------------------------------------------------------------------------------------------
+# These take logits in fp32, bf16 or fp16 and compute in fp32 and double.
+_ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+TopLogits = collections.namedtuple("TopLogits", "values index lse temperature")
+TopLogits.__doc__ = """What a teacher hands over per row: its k largest logits (largest first), their token ids (int64) and the log-sum-exp
+of all its logits at `temperature` (fp32; None where only the list is known)."""
+
+
+def _on_device(first, *rest):
+    """The raw stream to launch on.  All tensors have to live on the current device: kernels are launched there."""
+    for t in (first,) + rest:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise _lib.NastHipError("nast_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
+        if t.device != first.device:
+            raise _lib.NastHipError(f"tensors on two devices: {first.device} and {t.device}")
+    if first.device.index != torch.cuda.current_device():
+        raise _lib.NastHipError(f"tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(first.device.index)
+
+
+def _row_dtype(t):
+    if t.dtype not in _ROW_DTYPES:
+        raise _lib.NastHipError(f"fp32, bf16 or fp16 logits expected, got {t.dtype}")
+    return _ROW_DTYPES[t.dtype]
+
+
+def _vocab_rows(t):
+    """(tensor to read, its nast_rows, number of rows) for logits [..., V]; up to three dimensions are read through their strides."""
+    if t.dim() == 0 or t.shape[-1] == 0:
+        raise _lib.NastHipError(f"logits with a vocabulary axis expected, got shape {tuple(t.shape)}")
+    if t.dim() == 1:
+        t = t.unsqueeze(0)
+    elif t.dim() > 3:
+        t = t.reshape(-1, t.shape[-1])
+    if t.numel() and t.shape[-1] == 1:
+        t = t.contiguous()                      # the stride of an axis of one element says nothing
+    r, rows = rows_of(t)
+    return t, r, rows
+
+
+def _workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _positive(temperature):
+    t = float(temperature)
+    if not 0 < t < 1e30:
+        raise _lib.NastHipError(f"temperature must be > 0 and finite, got {t}")
+    return t
+
+
+def top_logits(logits, k, temperature=1.0):
+    """The k largest logits of every row of logits [..., V] and the row's log-sum-exp at `temperature`: TopLogits with values
+    [..., k] (the logits' type, largest first, ties to the lower id, NaN above everything), index [..., k] int64, lse [...] fp32.
+    1 <= k <= min(256, V).  No gradient flows: this is the teacher's side."""
+    logits = logits.detach()
+    stream, dtype, temperature, k = _on_device(logits), _row_dtype(logits), _positive(temperature), int(k)
+    x, r, rows = _vocab_rows(logits)
+    V = x.shape[-1]
+    if not 1 <= k <= min(256, V):
+        raise _lib.NastHipError(f"k={k} must lie in 1..256 and not exceed the vocabulary of {V}")
+    lead = logits.shape[:-1]
+    values = torch.empty(*lead, k, device=x.device, dtype=x.dtype)
+    index = torch.empty(*lead, k, device=x.device, dtype=torch.int64)
+    lse = torch.empty(lead, device=x.device, dtype=F32)
+    ws = _workspace(load().nast_top_logits_workspace_bytes(rows, V, k, dtype), x)
+    call("nast_top_logits", _p(x), dtype, r, _p(values), _p(index), _p(lse), rows, V, k, temperature, _p(ws), stream)
+    return TopLogits(values, index, lse, temperature)
+
+
+def _teacher_list(lead, top, temperature, tail):
+    """(values, index, lse or None) of a TopLogits, checked against the rows it belongs to."""
+    values, index, lse = top.values.detach(), top.index, top.lse
+    if values.dim() == 0 or tuple(values.shape[:-1]) != tuple(lead) or index.shape != values.shape:
+        raise _lib.NastHipError(f"teacher's list: values {tuple(values.shape)} and index {tuple(index.shape)} for rows {tuple(lead)}")
+    if not 1 <= values.shape[-1] <= 256:
+        raise _lib.NastHipError(f"a teacher's list has 1 to 256 slots, not {values.shape[-1]}")
+    if index.dtype != torch.int64:
+        raise _lib.NastHipError(f"int64 token ids expected, got {index.dtype}")
+    _row_dtype(values)
+    if not tail:
+        return _c(values), _c(index), None
+    if lse is None or lse.dtype != F32 or tuple(lse.shape) != tuple(lead):
+        raise _lib.NastHipError("tail=True needs the teacher's log-sum-exp, fp32, one per row")
+    if top.temperature != temperature:
+        raise _lib.NastHipError(f"the teacher's log-sum-exp was taken at temperature {top.temperature}, not {temperature}")
+    return _c(values), _c(index), _c(lse.detach())
+
+
+def _distill_fwd(x, r, rows, dtype, teacher, temperature, stream):
+    """-> loss [rows] fp32, stats [rows, 6] double"""
+    values, index, lse = teacher
+    V, K = x.shape[-1], values.shape[-1]
+    loss = torch.empty(rows, device=x.device, dtype=F32)
+    stats = torch.empty(rows, 6, device=x.device, dtype=torch.float64)
+    ws = _workspace(load().nast_top_distill_workspace_bytes(rows, V, dtype), x)
+    call("nast_top_distill_fwd", _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), K, _p(lse), _p(loss), _p(stats), rows, V,
+         temperature, _p(ws), stream)
+    return loss, stats
+
+
+def _distill_bwd(g, x, r, rows, dtype, values, index, stats, temperature, stream):
+    """-> d loss / d logits, contiguous, in the logits' type"""
+    V, K = x.shape[-1], values.shape[-1]
+    gx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    call("nast_top_distill_bwd", _p(g), _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), K, _p(stats), _p(gx), Rows(V, 0, 0),
+         rows, V, temperature, stream)
+    return gx
+
+
+class TopDistillFn(torch.autograd.Function):
+    """KL(teacher || student) per row, the teacher known by its top logits; one pass over the logits each way."""
+
+    @staticmethod
+    def forward(ctx, logits, top, temperature, tail):
+        teacher = _teacher_list(logits.shape[:-1], top, temperature, tail)
+        stream, dtype = _on_device(logits, *teacher), _row_dtype(logits)
+        x, r, rows = _vocab_rows(logits)
+        loss, stats = _distill_fwd(x, r, rows, dtype, teacher, temperature, stream)
+        ctx.save_for_backward(logits, teacher[0], teacher[1], stats)
+        ctx.temperature = temperature
+        return loss.view(logits.shape[:-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits, values, index, stats = ctx.saved_tensors
+        x, r, rows = _vocab_rows(logits)
+        gx = _distill_bwd(_c(g).view(-1), x, r, rows, _ROW_DTYPES[x.dtype], values, index, stats, ctx.temperature, _on_device(logits, g))
+        return gx.view(logits.shape), None, None, None
+
+
+def top_distill(logits, top, temperature=1.0, tail=False):
+    """Distillation loss [...] (fp32) of a student's logits [..., V] against a teacher's TopLogits [..., K], with gradient to the logits.
+
+      p_j = exp(t_j / T - c),  q = softmax(logits / T),  loss = sum_j p_j (log p_j - log q_{id_j})
+
+    tail=False: c normalises the list itself.  tail=True: c = top.lse (taken at the same T), and what the list leaves out is one more
+    class, with the teacher's 1 - sum p_j against the student's probability of every token outside the list.
+    Slots whose id lies outside [0, V) (-1: the list ends early) or whose logit is -inf are unused; a row without a used slot has
+    loss 0 and gradient 0; an id in two slots counts in both.  Multiply by T * T for gradients of the usual scale."""
+    return TopDistillFn.apply(logits, top, _positive(temperature), bool(tail))
+
+
+class GeneratorDistillFn(torch.autograd.Function):
+    """top_distill of (x W^T + b) as one node: Generator (transformer.py:213-214) and the distillation loss on its logits."""
+
+    @staticmethod
+    def forward(ctx, x, W, b, temperature, top, tail):
+        _chk(x, W, b)
+        teacher = _teacher_list(x.shape[:-1], top, temperature, tail)
+        stream = _on_device(x, W, b, *teacher)
+        x2 = _c(x).view(-1, x.shape[-1])
+        V = W.shape[0]
+        y = torch.empty(x2.shape[0], V, device=x.device, dtype=F32)
+        if x2.shape[0]:
+            gemm([d_fwd(x2, W, y, bias=b)])
+        loss, stats = _distill_fwd(y, Rows(V, 0, 0), y.shape[0], 0, teacher, temperature, stream)
+        ctx.save_for_backward(x2, W, y, teacher[0], teacher[1], stats)
+        ctx.params = live(W, b)
+        ctx.temperature, ctx.xshape = temperature, x.shape
+        return loss.view(x.shape[:-1])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        x2, W, y, values, index, stats = ctx.saved_tensors
+        gl = _distill_bwd(_c(g).view(-1), y, Rows(W.shape[0], 0, 0), y.shape[0], 0, values, index, stats, ctx.temperature, _on_device(y, g))
+        (dW, db), (rW, rb) = grad_buffers(list(ctx.params))
+        dx = torch.empty_like(x2)
+        if x2.shape[0]:
+            gemm([d_dgrad([gl], [W], dx)] + wgrad_descs(gl, x2, dW, db))
+        grads_written(ctx.params)
+        return dx.view(ctx.xshape), rW, rb, None, None, None
+
+
+def generator_distill(x, W, b, temperature, top, tail=False):
+    """top_distill(x W^T + b, top, temperature, tail) with gradients to x, W and b."""
+    return GeneratorDistillFn.apply(x, W, b, _positive(temperature), top, bool(tail))
+
+
+def verify_draft(target, tokens, u, E, draft=None, lengths=None, temperature=1.0):
+    """Which drafted tokens a target model lets stand, and the token behind them (speculative sampling): the tokens that come out are
+    distributed as if the target had drawn each of them.  -> (out [B, N + 1] int64, accepted [B] int64)
+
+      target [B, N + 1, V]  the target's logits at the place of every draft and behind the last
+      tokens [B, N] int64   the drafts, `lengths` [B] int64 how many of each sequence count (None: all N)
+      draft [B, N, V]       the logits they were drawn from (same type as target); None: drafts without probabilities, q(d) = 1
+      u [B, N] fp32         uniforms in [0, 1);   E [B, V] fp32  Exp(1) draws
+
+    With p_i, q_i the softmax of the rows over `temperature`, draft i stands while u_i q_i(d_i) < p_i(d_i) (and q_i(d_i) > 0).  out
+    holds the drafts that stand, then argmax (p_i - q_i)+ / E at the first that falls (p_N / E if none does), then -1.  A target row
+    without a distribution (a NaN, a +inf, nothing but -inf) lets nothing stand and gives -1."""
+    target, draft = target.detach(), None if draft is None else draft.detach()
+    stream, dtype, temperature = _on_device(target, tokens, u, E, draft, lengths), _row_dtype(target), _positive(temperature)
+    if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
+        raise _lib.NastHipError(f"target logits [B, N + 1, V] expected, got {tuple(target.shape)}")
+    B, N, V = target.shape[0], target.shape[1] - 1, target.shape[2]
+    for name, t, shape, kind in (("tokens", tokens, (B, N), torch.int64), ("u", u, (B, N), F32), ("E", E, (B, V), F32),
+                                 ("draft", draft, (B, N, V), target.dtype), ("lengths", lengths, (B,), torch.int64)):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != kind):
+            raise _lib.NastHipError(f"{name}: {shape} {kind} expected, got {tuple(t.shape)} {t.dtype}")
+    target, draft = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (target, draft))
+    tokens, u, E, lengths = (None if t is None else _c(t) for t in (tokens, u, E, lengths))
+    out = torch.empty(B, N + 1, device=target.device, dtype=torch.int64)
+    accepted = torch.empty(B, device=target.device, dtype=torch.int64)
+    ws = _workspace(load().nast_verify_draft_workspace_bytes(B, N, V, dtype), target)
+    call("nast_verify_draft", _p(target), target.stride(0), target.stride(1), _p(draft), *((0, 0) if draft is None else draft.stride()[:2]),
+         dtype, _p(tokens), _p(u), _p(E), _p(lengths), _p(out), _p(accepted), B, N, V, temperature, _p(ws), stream)
+    return out, accepted
 
 
 def first_eos_length(tokens, eos):

@@ -231,6 +231,15 @@ class Generator(nn.Module):
         """-forward(x, temperature).gather(-1, tokens): the NLLLoss(reduction='none') of seq2seq.py:453 fused in."""
         return ops.generator_nll(x, self.proj.weight, self.proj.bias, temperature, tokens)
 
+    def top(self, x, temperature, k):
+        """A teacher's side: the k largest logits of every position and their log-sum-exp (ops.TopLogits), no gradient."""
+        with torch.no_grad():
+            return ops.top_logits(ops.linear(x, self.proj.weight, self.proj.bias), k, temperature)
+
+    def distill(self, x, temperature, top, tail=False):
+        """A student's side: the loss of every position against a teacher's ops.TopLogits (ops.top_distill)."""
+        return ops.generator_distill(x, self.proj.weight, self.proj.bias, temperature, top, tail)
+
 
 class Decoder(nn.Module):
     lazy_log_softmax = True     # packed log-probs of the transfer pass leave the generator as logits (see _forward_packed)
@@ -241,15 +250,19 @@ class Decoder(nn.Module):
         self.norm = LayerNorm(d_model)
         self.generator = Generator(d_model, vocab_size)
 
-    def forward(self, x, memory, src_mask, tgt_mask, temperature, skip_first=False, nll_targets=None, packed_out=False):
+    def forward(self, x, memory, src_mask, tgt_mask, temperature, skip_first=False, nll_targets=None, packed_out=False,
+                teacher_top=None, teacher_tail=False):
         """transformer.py:180-188.  skip_first=True returns log-probs for positions 1.. only
         (what StyleTransformer keeps, transformer.py:103) without computing row 0; with nll_targets [B, n-1]
-        the per-token negative log-likelihood of those tokens is returned instead of the log-probs."""
+        the per-token negative log-likelihood of those tokens is returned instead of the log-probs, with teacher_top (an
+        ops.TopLogits of [B, n-1, K]) the per-token distillation loss (ops.top_distill)."""
+        if teacher_top is not None and (nll_targets is not None or not skip_first or packed_out):
+            raise ops._lib.NastHipError("teacher_top goes with skip_first and neither nll_targets nor packed_out")
         assert x.size(1) == tgt_mask.size(-1)
         dk = x.shape[-1] // self.layers[0].self_attn.h
         pt, pm = ops.packed_of(tgt_mask, x, dk), ops.packed_of(src_mask, memory, dk)
         if pt is not None and pm is not None and skip_first:
-            return self._forward_packed(x, memory, pt, pm, temperature, nll_targets, packed_out)
+            return self._forward_packed(x, memory, pt, pm, temperature, nll_targets, packed_out, teacher_top, teacher_tail)
         y = x
         memory = ops.shared_kv(memory)      # one gradient buffer for all layers' cross-attention (ops.SharedKVFn)
         for layer in self.layers:
@@ -260,10 +273,12 @@ class Decoder(nn.Module):
             if nll_targets is not None:
                 assert nll_targets.shape == (B, n - 1)
                 return self.generator.nll(z, temperature, nll_targets).view(B, n - 1)
+            if teacher_top is not None:
+                return self.generator.distill(z.view(B, n - 1, d), temperature, teacher_top, teacher_tail)
             return self.generator(z, temperature).view(B, n - 1, -1)
         return self.generator(self.norm(y), temperature)
 
-    def _forward_packed(self, x, memory, pt, pm, temperature, nll_targets, packed_out=False):
+    def _forward_packed(self, x, memory, pt, pm, temperature, nll_targets, packed_out=False, teacher_top=None, teacher_tail=False):
         """The same stack on the real rows only (ops.PackedSeq); positions 1.. of every sentence are kept."""
         B, n, d = x.shape
         y, mem = ops.pack_rows(x, pt), ops.pack_rows(memory, pm)
@@ -279,6 +294,13 @@ class Decoder(nn.Module):
             tok = nll_targets.reshape(-1).index_select(0, sub.idx_p)
             nll = self.generator.nll(z, temperature, tok).view(-1)[:sub.total]
             return torch.zeros(B * (n - 1), device=x.device, dtype=nll.dtype).index_copy(0, sub.idx, nll).view(B, n - 1)
+        if teacher_top is not None:                             # padded positions come back as 0
+            if tuple(teacher_top.index.shape[:-1]) != (B, n - 1):
+                raise ops._lib.NastHipError(f"teacher_top: lists [{B}, {n - 1}, K] expected, got {tuple(teacher_top.index.shape)}")
+            pick = lambda t: None if t is None else t.flatten(0, 1).index_select(0, sub.idx_p)
+            top = ops.TopLogits(pick(teacher_top.values), pick(teacher_top.index), pick(teacher_top.lse), teacher_top.temperature)
+            loss = self.generator.distill(z, temperature, top, teacher_tail)[:sub.total]
+            return torch.zeros(B * (n - 1), device=x.device, dtype=loss.dtype).index_copy(0, sub.idx, loss).view(B, n - 1)
         if packed_out:                                          # log-probs of the real positions only: [sub.rows, V]
             # (at temperature 1 the log-sum-exp pass is left to the consumer: Seq2seq._approx_packed's Gumbel-softmax does
             # not need it, ops.GeneratorFn)
@@ -339,10 +361,12 @@ class StyleTransformer(nn.Module):
 
     def forward(self, inp_tokens, inp_lengths, gold_tokens, gold_lengths, style,
                 generate=False, differentiable_decode=False, temperature=1.0, *, use_inference_z, nll_targets=None,
-                packed_log_probs=False):
+                packed_log_probs=False, teacher_top=None, teacher_tail=False):
         """transformer.py:48-103 -> (log_probs[:,1:], tgt_lengths, length_loss, gen_error, allpos).
         Extension: nll_targets [B,T] int64 -> the first result is -log_probs[:,1:].gather(-1, nll_targets) [B,T]
-        (what seq2seq.py:453 / :504 compute from the log-probs), without materialising their gradient."""
+        (what seq2seq.py:453 / :504 compute from the log-probs), without materialising their gradient; teacher_top, an
+        ops.TopLogits of [B,T,K] -> the distillation loss [B,T] of every position against a teacher's top logits
+        (ops.top_distill at this temperature, teacher_tail its tail)."""
         batch_size = inp_tokens.size(0)
         max_enc_len = inp_tokens.size(1)
         if self.check_lengths and not ops.FIXED_WIDTH:
@@ -386,7 +410,7 @@ class StyleTransformer(nn.Module):
         # packed_log_probs (extension): when the decoder runs on packed rows, hand the log-probs back as ops.PackedSoft
         # (real positions only) instead of the padded [B, T, V] tensor
         log_probs = self.decoder(dec_input_emb, memory, src_mask, tgt_mask, temperature, skip_first=True,
-                                 nll_targets=nll_targets, packed_out=packed_log_probs)
+                                 nll_targets=nll_targets, packed_out=packed_log_probs, teacher_top=teacher_top, teacher_tail=teacher_tail)
         return log_probs, tgt_lengths, length_loss, gen_error, allpos
 
 

@@ -69,6 +69,18 @@ def straight_max(logits, dim=-1, allow_gradient=False):
     return y_hard, y_soft
 
 
+def verify_draft(target_logits, draft_tokens, draft_logits=None, lengths=None, tau=1):
+    """-> (tokens [B, N + 1], accepted [B]): ops.verify_draft with the uniforms [B, N] and then the Exp(1) draws [B, V] taken from
+    inject_noise, or drawn by torch's generator."""
+    B, n, V = target_logits.shape
+    u, E = _next_noise(), _next_noise()
+    if u is None:
+        u = torch.rand(B, n - 1, device=target_logits.device)
+    if E is None:
+        E = torch.empty(B, V, device=target_logits.device).exponential_()
+    return ops.verify_draft(target_logits, draft_tokens, u, E, draft_logits, lengths, tau)
+
+
 def onehot(sent, vocab_size):
     return torch.zeros(*sent.shape, vocab_size, device=sent.device).scatter_(-1, sent.unsqueeze(-1), 1.0)
 
