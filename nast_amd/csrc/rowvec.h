@@ -5,23 +5,23 @@
 
 #include "common.h"
 
-// One struct per storage type: EPV elements in 16 bytes, their conversion to fp32 (exact) and back (to nearest even).
+// One struct per storage type: EPV elements in 16 bytes, their conversion to fp32 (exact) and back (to nearest even); the low
+// KEY_ZEROS bits of an fp32 mantissa that no value of the type uses.
 struct RowF32 {
   using store = float;
-  static constexpr int EPV = 4;
-  static constexpr float neg_inf() { return -INFINITY; }
+  static constexpr int EPV = 4, KEY_ZEROS = 0;
   static __device__ __forceinline__ float get(store v) { return v; }
   static __device__ __forceinline__ store put(float v) { return v; }
 };
 struct RowBF16 {
   using store = __bf16;
-  static constexpr int EPV = 8;
+  static constexpr int EPV = 8, KEY_ZEROS = 16;
   static __device__ __forceinline__ float get(store v) { return (float)v; }
   static __device__ __forceinline__ store put(float v) { return (store)v; }
 };
 struct RowF16 {
   using store = _Float16;
-  static constexpr int EPV = 8;
+  static constexpr int EPV = 8, KEY_ZEROS = 13;
   static __device__ __forceinline__ float get(store v) { return (float)v; }
   static __device__ __forceinline__ store put(float v) { return (store)v; }
 };
@@ -32,48 +32,44 @@ union RowVec {
   typename D::store e[D::EPV];
 };
 
-// Elements [lo, hi) of a row in vector slots: slot s holds elements first + s * EPV ..., where `first` <= lo is the element
-// whose address is 16-byte aligned.  The slots at the two ends may stick out of [lo, hi); those are read and written element
-// by element, what lies outside reads as -inf and is never touched.
+// 16 bytes from any element: global_load_dwordx4 takes any alignment on this target
+typedef uint32_t raw16_any __attribute__((ext_vector_type(4), aligned(2)));
 template <class D>
-struct RowSlots {
-  int first, lo, hi, n;
-  __device__ __forceinline__ RowSlots(const typename D::store* p, int lo_, int hi_) : lo(lo_), hi(hi_) {
-    const int lead = (int)((reinterpret_cast<uintptr_t>(p + lo_) & 15) / sizeof(typename D::store));
-    first = lo_ - lead;
-    n = (hi_ - first + D::EPV - 1) / D::EPV;
+__device__ __forceinline__ RowVec<D> load16(const typename D::store* p) {
+  const raw16_any q = *reinterpret_cast<const raw16_any*>(p);
+  RowVec<D> v;
+  v.raw = make_uint4(q.x, q.y, q.z, q.w);
+  return v;
+}
+
+// Elements [lo, hi) of a row: a body of whole 16-byte aligned vectors, slot s at element body + s * EPV, and at most EPV - 1 elements
+// in front of it and behind it.  Those are dealt out one to a thread (threads 0.. and 64..), so that no vector has holes.
+template <class D>
+struct RowSpan16 {
+  int lo, hi, body, n, tail;
+  __device__ __forceinline__ RowSpan16(const typename D::store* p, int lo_, int hi_) : lo(lo_), hi(hi_) {
+    const int lead = (int)((0 - reinterpret_cast<uintptr_t>(p + lo_)) & 15) / (int)sizeof(typename D::store);
+    body = min(lo_ + lead, hi_);
+    n = (hi_ - body) / D::EPV;
+    tail = body + n * D::EPV;
   }
-  __device__ __forceinline__ int elem(int s) const { return first + s * D::EPV; }
-  __device__ __forceinline__ bool whole(int s) const { return elem(s) >= lo && elem(s) + D::EPV <= hi; }
+  __device__ __forceinline__ int elem(int s) const { return body + s * D::EPV; }
   __device__ __forceinline__ RowVec<D> load(const typename D::store* p, int s) const {
     RowVec<D> v;
-    const int e0 = elem(s);
-    if (whole(s)) {
-      v.raw = *reinterpret_cast<const uint4*>(p + e0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < D::EPV; ++i) v.e[i] = (e0 + i >= lo && e0 + i < hi) ? p[e0 + i] : D::put(-INFINITY);
-    }
+    v.raw = *reinterpret_cast<const uint4*>(p + body + s * D::EPV);
     return v;
+  }
+  // the element thread t has to look after besides its slots, or -1
+  __device__ __forceinline__ int edge(int t) const {
+    if (t < body - lo) return lo + t;
+    return t >= 64 && t - 64 < hi - tail ? tail + (t - 64) : -1;
   }
 };
 
-// exp(t / T) = 2^(t * log2(e) / T) with the factor held in two floats: one rounding of the product's magnitude, ~1e-7 relative in
-// the result for t / T > -30 instead of ~1e-6.  t is a difference to a maximum: <= 0 or -inf or NaN.  (The low part is taken of a
-// clamped t: -inf times a low part of 0 or of the other sign would be NaN.)
-struct ExpScale {
-  float hi, lo;
-};
-static inline ExpScale exp_scale(double temp) {
-  const double c = 1.4426950408889634 / temp;
-  ExpScale e;
-  e.hi = (float)c;
-  e.lo = (float)(c - (double)e.hi);
-  return e;
-}
-__device__ __forceinline__ float exp_t(float t, ExpScale c) {
-  return __builtin_amdgcn_exp2f(__builtin_fmaf(t, c.hi, fmaxf(t, -1e30f) * c.lo));
-}
+// exp(t / T) as 2^(t * c), c = log2(e) / T rounded to fp32.  t is a difference to a maximum (<= 0 or -inf or NaN).  The product's
+// rounding and c's make the result wrong by at most |t * c| * 2^-23 * ln 2 relative: 4e-6 where it is 2^-40, 1e-7 where it is near 1.
+static inline float exp_scale(double temp) { return (float)(1.4426950408889634 / temp); }
+__device__ __forceinline__ float exp_t(float t, float c) { return __builtin_amdgcn_exp2f(t * c); }
 
 // Sum of exponentials relative to a maximum.  The maximum starts at the lowest finite value, so that no -inf is subtracted from
 // -inf: a row of -inf ends with s = 0 (log-sum-exp -inf), a row of the type's lowest value counts as any other row.  A NaN or
@@ -81,22 +77,56 @@ __device__ __forceinline__ float exp_t(float t, ExpScale c) {
 struct MaxSum {
   float m, s;
 };
-template <class D>
-__device__ __forceinline__ void fold(MaxSum& a, const RowVec<D>& v, ExpScale c) {
-  float f[D::EPV], top = -FLT_MAX;
+// U vectors at a time: one comparison with the running maximum and at most one rescaling for all of them
+template <class D, int U>
+__device__ __forceinline__ void fold(MaxSum& a, const RowVec<D> (&v)[U], float c) {
+  float top = -FLT_MAX;
 #pragma unroll
-  for (int i = 0; i < D::EPV; ++i) {
-    f[i] = D::get(v.e[i]);
-    top = fmaxf(top, f[i]);
-  }
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < D::EPV; ++i) top = fmaxf(top, D::get(v[u].e[i]));
   if (top > a.m) {
     a.s *= exp_t(a.m - top, c);
     a.m = top;
   }
-  float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < D::EPV; ++i) s += exp_t(f[i] - a.m, c);
-  a.s += s;
+  for (int u = 0; u < U; ++u) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < D::EPV; ++i) s += exp_t(D::get(v[u].e[i]) - a.m, c);
+    a.s += s;
+  }
+}
+__device__ __forceinline__ void fold_one(MaxSum& a, float f, float c) {
+  if (f > a.m) {
+    a.s *= exp_t(a.m - f, c);
+    a.m = f;
+  }
+  a.s += exp_t(f - a.m, c);
+}
+
+// a thread's share of elements [lo, hi) of a row
+template <class D, int NT>
+__device__ __forceinline__ MaxSum span_max_sum(const typename D::store* p, int lo, int hi, float c) {
+  constexpr int U = 4;
+  const RowSpan16<D> rs(p, lo, hi);
+  MaxSum a{-FLT_MAX, 0.f};
+  for (int base = threadIdx.x; base < rs.n; base += NT * U) {
+    RowVec<D> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (base + NT * u < rs.n) {
+        v[u] = rs.load(p, base + NT * u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(-INFINITY);
+      }
+    }
+    fold<D, U>(a, v, c);
+  }
+  const int e = rs.edge(threadIdx.x);
+  if (e >= 0) fold_one(a, D::get(p[e]), c);
+  return a;
 }
 
 struct MaxSumD {
@@ -114,7 +144,7 @@ __device__ __forceinline__ double wave_max_d(double v) {
 }
 // every thread gets the block's pair; red: LDS of 2 * NT / 64 doubles; two barriers
 template <int NT>
-__device__ __forceinline__ MaxSumD block_max_sum(MaxSum a, ExpScale c, double* red) {
+__device__ __forceinline__ MaxSumD block_max_sum(MaxSum a, float c, double* red) {
   const float wm = wave_max(a.m);
   const double ws = wave_sum_d((double)(a.s * exp_t(a.m - wm, c)));
   const int w = threadIdx.x >> 6;
@@ -138,6 +168,19 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
   const uint32_t k = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
   return v != v ? 0xffffffffu : k;
+}
+
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __builtin_bit_cast(float, (k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+
+// Into how many chunks a row of V elements is cut: as few as `most` elements a chunk allow; more while rows * chunks is below 512
+// workgroups (two a compute unit), but none shorter than `least`.
+static inline int row_chunks(int rows, int V, int most, int least) {
+  const int need = (V + most - 1) / most;
+  int n = rows > 0 && rows < 512 ? (512 + rows - 1) / rows : 1;
+  if (n > V / least) n = V / least;
+  return n > need ? n : need;
 }
 
 static inline int row_size(int dtype) { return dtype == NAST_F32 ? 4 : 2; }

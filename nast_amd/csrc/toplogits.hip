@@ -11,87 +11,359 @@
 // top logits
 // ---------------------------------------------------------------------------------------------
 #define TOP_MAX_K 256
+#define TOP_CAND 512              // candidates a workgroup ranks
+#define TOP_MAX_LIST 16384        // entries the join of a row's chunks takes
 
-// One workgroup per row.  Elements are ordered by (key, lower id first): the 64-bit number key << 32 | ~id differs for any two
-// elements of a row.  The k-th largest such number is found by bisection over its bits, counting the elements at or above a
-// candidate; the k elements at or above it are collected and ranked by comparison with each other.
-template <class D>
-__global__ __launch_bounds__(256) void nast_top_logits_kernel(const typename D::store* __restrict__ x, nast_rows xr,
-                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
-                                                              float* __restrict__ lse, int V, int k, double inv_temp, ExpScale c) {
-  __shared__ double red[8];
-  __shared__ int cnt[4];
-  __shared__ uint64_t cand[TOP_MAX_K];
-  __shared__ int n_cand;
-  const int64_t r = blockIdx.x;
-  const typename D::store* p = x + row_offset(r, xr);
-  const RowSlots<D> rs(p, 0, V);
-  MaxSum a{-FLT_MAX, 0.f};
-  for (int s = threadIdx.x; s < rs.n; s += 256) fold<D>(a, rs.load(p, s), c);
-  const MaxSumD t = block_max_sum<256>(a, c, red);
-  if (threadIdx.x == 0) lse[r] = (float)(t.m * inv_temp + log(t.s));
+// Elements are ordered by value, ties to the lower id: entry = key << 32 | ~id is one 64-bit number per element, no two alike, 0 is
+// no element.
+__device__ __forceinline__ uint64_t top_entry(float f, int e) { return ((uint64_t)order_key(f) << 32) | (uint32_t)~e; }
+__device__ __forceinline__ int entry_id(uint64_t o) { return (int)~(uint32_t)o; }
 
-  uint64_t bound = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t mid = bound | (1ull << bit);
-    int n = 0;
-    for (int s = threadIdx.x; s < rs.n; s += 256) {
-      const RowVec<D> v = rs.load(p, s);
-#pragma unroll
-      for (int i = 0; i < D::EPV; ++i) {
-        const int e = rs.elem(s) + i;
-        const uint64_t o = ((uint64_t)order_key(D::get(v.e[i])) << 32) | (uint32_t)~e;
-        n += (e >= 0 && e < V && o >= mid) ? 1 : 0;
-      }
-    }
-    n = (int)wave_sum((float)n);       // <= V < 2^24 per wavefront: exact in fp32
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) cnt[threadIdx.x >> 6] = n;
-    __syncthreads();
-    if (cnt[0] + cnt[1] + cnt[2] + cnt[3] >= k) bound = mid;
-  }
-  if (threadIdx.x == 0) n_cand = 0;
-  __syncthreads();
-  for (int s = threadIdx.x; s < rs.n; s += 256) {
-    const RowVec<D> v = rs.load(p, s);
-#pragma unroll
-    for (int i = 0; i < D::EPV; ++i) {
-      const int e = rs.elem(s) + i;
-      const uint64_t o = ((uint64_t)order_key(D::get(v.e[i])) << 32) | (uint32_t)~e;
-      if (e >= 0 && e < V && o >= bound) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at < TOP_MAX_K) cand[at] = o;
-      }
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < k; i += 256) {
+// Each of n <= TOP_CAND distinct entries in LDS is written at its rank among them, up to rank k.
+template <int NT, class F>
+__device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, F&& out) {
+  for (int i = threadIdx.x; i < n; i += NT) {
     const uint64_t o = cand[i];
     int rank = 0;
-    for (int j = 0; j < k; ++j) rank += cand[j] > o ? 1 : 0;
-    const int e = (int)~(uint32_t)o;
-    index[r * k + rank] = e;
-    values[r * k + rank] = p[e];
+    for (int j = 0; j < n; ++j) rank += cand[j] > o ? 1 : 0;
+    if (rank < k) out(rank, o);
   }
 }
 
-extern "C" int64_t nast_top_logits_workspace_bytes(int rows, int V, int k, int dtype) { return 0; }
+template <int NT>
+__device__ __forceinline__ int block_count(int n, int* cnt) {   // n <= 2^16 a thread; two barriers
+  n = (int)wave_sum((float)n);                                  // <= 2^22: exact in fp32
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) cnt[threadIdx.x >> 6] = n;
+  __syncthreads();
+  int t = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) t += cnt[i];
+  return t;
+}
+
+// One workgroup per chunk of a row, the chunk in registers: NV vectors a thread (and an edge element), read from memory once.
+//
+// The k-th largest of the maxima of disjoint groups of elements is a lower bound of the k-th largest element.  Each thread keeps the
+// maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and every
+// wavefront finds a bound among them by bisection on the upper half of the order key, content with up to k + k/4 + 8 groups at
+// or above it.  Vectors whose maximum reaches the bound are looked through again; what is found there (a little more than k
+// elements where they lie at random) is ranked by counting.  Where more than TOP_CAND elements reach the bound (many equal
+// values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the
+// registers, and equal elements are taken in the order of their ids.
+template <class D, int NV>
+__global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
+                                                             typename D::store* __restrict__ values, int64_t* __restrict__ index,
+                                                             float* __restrict__ lse, uint64_t* __restrict__ lists,
+                                                             MaxSumD* __restrict__ parts, int V, int k, int chunk, int n_chunk,
+                                                             double inv_temp, float c) {
+  constexpr int G = NV >= 4 ? 4 : 1;
+  __shared__ float gmax[256 * G];
+  __shared__ uint64_t cand[TOP_CAND];
+  __shared__ double red[4];
+  __shared__ int cnt[4];
+  __shared__ int n_cand;
+  const int64_t r = blockIdx.x / n_chunk;
+  const int tid = threadIdx.x, lane = tid & 63, lo = (int)(blockIdx.x % n_chunk) * chunk, hi = min(V, lo + chunk);
+  const typename D::store* p = x + row_offset(r, xr);
+  const RowSpan16<D> rs(p, lo, hi);
+  const int kk = min(k, hi - lo);
+  RowVec<D> v[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * 256 < rs.n) {
+      if (i * 256 + tid < rs.n) v[i] = rs.load(p, i * 256 + tid);
+      else
+#pragma unroll
+        for (int j = 0; j < D::EPV; ++j) v[i].e[j] = D::put(-INFINITY);
+    }
+  }
+  const int ee = rs.edge(tid);
+  const float ef = ee >= 0 ? D::get(p[ee]) : -INFINITY;
+  if (tid == 0) n_cand = 0;
+
+  float vm[NV], g[G];
+#pragma unroll
+  for (int i = 0; i < G; ++i) g[i] = -INFINITY;
+  g[0] = fmaxf(g[0], ef);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    vm[i] = -INFINITY;
+    if (i * 256 < rs.n) {
+#pragma unroll
+      for (int j = 0; j < D::EPV; ++j) vm[i] = fmaxf(vm[i], D::get(v[i].e[j]));
+      g[i % G] = fmaxf(g[i % G], vm[i]);
+    }
+  }
+  const int groups = G > 1 && k > 64 ? G : 1;
+  if (groups > 1) {
+#pragma unroll
+    for (int i = 0; i < G; ++i) gmax[i * 256 + tid] = g[i];
+  } else {
+#pragma unroll
+    for (int i = 1; i < G; ++i) g[0] = fmaxf(g[0], g[i]);
+    gmax[tid] = g[0];
+  }
+  __syncthreads();
+
+  // the bound, by every wavefront for itself
+  float m = -INFINITY, least = INFINITY, thr;
+  uint32_t gk[4 * G];
+#pragma unroll
+  for (int i = 0; i < 4 * G; ++i) {
+    gk[i] = 0;
+    if (i < 4 * groups) {
+      const float f = gmax[i * 64 + lane];
+      m = fmaxf(m, f);
+      least = fminf(least, f);
+      gk[i] = order_key(f) >> 16;
+    }
+  }
+  m = wave_max(m);
+  least = -wave_max(-least);
+  {
+    uint32_t b0 = order_key(least) >> 16, b1 = (order_key(m) >> 16) + 1;
+    while (b1 - b0 > 1) {
+      const uint32_t mid = (b0 + b1) >> 1;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < 4 * G; ++i)
+        if (i < 4 * groups) n += __popcll(__ballot(gk[i] >= mid));
+      if (n >= kk) {
+        b0 = mid;
+        if (n <= kk + kk / 4 + 8) break;
+      } else {
+        b1 = mid;
+      }
+    }
+    b0 <<= 16;
+    thr = b0 < 0x00800000u ? -INFINITY : key_value(b0);
+  }
+
+  if (ef >= thr && ee >= 0) {
+    const int at = atomicAdd(&n_cand, 1);
+    if (at < TOP_CAND) cand[at] = top_entry(ef, ee);
+  }
+  uint32_t hits = 0;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (i * 256 < rs.n) hits |= (vm[i] >= thr && i * 256 + tid < rs.n ? 1u : 0u) << i;
+  while (hits) {
+    const int s = (__ffs(hits) - 1) * 256 + tid;
+    hits &= hits - 1;
+    const RowVec<D> w = rs.load(p, s);
+    for (int j = 0; j < D::EPV; ++j) {
+      const float f = D::get(w.e[j]);
+      if (f >= thr) {
+        const int at = atomicAdd(&n_cand, 1);
+        if (at < TOP_CAND) cand[at] = top_entry(f, rs.elem(s) + j);
+      }
+    }
+  }
+
+  m = fmaxf(m, -FLT_MAX);
+  float sum = exp_t(ef - m, c);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (i * 256 < rs.n) {
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < D::EPV; ++j) t += exp_t(D::get(v[i].e[j]) - m, c);
+      sum += t;
+    }
+  }
+  const double ws = wave_sum_d((double)sum);
+  if (lane == 0) red[tid >> 6] = ws;
+  __syncthreads();
+  const double s = (red[0] + red[1]) + (red[2] + red[3]);
+  int n = n_cand;
+
+  if (s != s || n > TOP_CAND) {
+    constexpr int SHIFT = D::KEY_ZEROS;
+    auto count = [&](uint64_t at_least) {                       // elements with key >> SHIFT at or above
+      int q = ee >= 0 && (order_key(ef) >> SHIFT) >= at_least ? 1 : 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (i * 256 + tid < rs.n)
+#pragma unroll
+          for (int j = 0; j < D::EPV; ++j) q += (order_key(D::get(v[i].e[j])) >> SHIFT) >= at_least ? 1 : 0;
+      return block_count<256>(q, cnt);
+    };
+    uint64_t b0 = 0, b1 = 1ull << (32 - SHIFT);
+    while (b1 - b0 > 1) {
+      const uint64_t mid = (b0 + b1) >> 1;
+      if (count(mid) >= kk) b0 = mid;
+      else b1 = mid;
+    }
+    const int need = kk - count(b0 + 1);                        // of those equal to the k-th
+    if (tid == 0) n_cand = 0;
+    __syncthreads();
+    int before = 0;
+    // pieces of ascending ids: head, the vectors one row of slots after the other, tail
+    for (int piece = -1; piece <= NV; ++piece) {
+      if (piece >= 0 && piece < NV && piece * 256 >= rs.n) continue;
+      uint64_t mine[D::EPV];
+      int same = 0;
+      uint32_t is_same = 0, is_more = 0;
+      if (piece == -1 || piece == NV) {
+        const bool here = ee >= 0 && (piece == -1) == (ee < rs.body);
+        const uint32_t key = order_key(ef) >> SHIFT;
+        mine[0] = top_entry(ef, ee);
+        is_same = here && key == b0 ? 1 : 0;
+        is_more = here && key > b0 ? 1 : 0;
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+          if (i == piece && i * 256 + tid < rs.n)
+#pragma unroll
+            for (int j = 0; j < D::EPV; ++j) {
+              const float f = D::get(v[i].e[j]);
+              const uint32_t key = order_key(f) >> SHIFT;
+              mine[j] = top_entry(f, rs.elem(i * 256 + tid) + j);
+              is_same |= (key == b0 ? 1u : 0u) << j;
+              is_more |= (key > b0 ? 1u : 0u) << j;
+            }
+      }
+      same = __popc(is_same);
+      int scan = same;                                          // inclusive over the wavefront
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int q = __shfl_up(scan, o, 64);
+        if (lane >= o) scan += q;
+      }
+      __syncthreads();
+      if (lane == 63) cnt[tid >> 6] = scan;
+      __syncthreads();
+      int place = before + scan - same;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < tid >> 6) place += cnt[i];
+        before += cnt[i];
+      }
+#pragma unroll
+      for (int j = 0; j < D::EPV; ++j) {
+        const bool eq = is_same >> j & 1;
+        if ((eq && place < need) || (is_more >> j & 1)) cand[atomicAdd(&n_cand, 1)] = mine[j];
+        place += eq ? 1 : 0;
+      }
+    }
+    __syncthreads();
+    n = kk;
+  }
+
+  if (n_chunk == 1) {
+    rank_out<256>(cand, n, k, [&](int rank, uint64_t o) {
+      index[r * k + rank] = entry_id(o);
+      values[r * k + rank] = D::put(key_value((uint32_t)(o >> 32)));
+    });
+    if (tid == 0) lse[r] = (float)((double)m * inv_temp + log(s));
+  } else {
+    uint64_t* l = lists + (int64_t)blockIdx.x * k;
+    rank_out<256>(cand, n, k, [&](int rank, uint64_t o) { l[rank] = o; });
+    for (int i = kk + tid; i < k; i += 256) l[i] = 0;
+    if (tid == 0) parts[blockIdx.x] = {(double)m, s};
+  }
+}
+
+// The lists of a row's chunks joined: 16 entries a thread, bisection until between k and TOP_CAND of them are left, ranks by counting.
+template <class D, int NT>
+__global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __restrict__ lists, const MaxSumD* __restrict__ parts,
+                                                           typename D::store* __restrict__ values, int64_t* __restrict__ index,
+                                                           float* __restrict__ lse, int k, int n_chunk, double inv_temp) {
+  __shared__ uint64_t cand[TOP_CAND];
+  __shared__ int cnt[NT / 64];
+  __shared__ int n_cand;
+  const int64_t r = blockIdx.x;
+  const int n = n_chunk * k;
+  uint64_t o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = i * NT + (int)threadIdx.x < n ? lists[r * n + i * NT + threadIdx.x] : 0;
+  if (threadIdx.x == 0) n_cand = 0;
+  uint64_t b0 = 1;
+  if (n > TOP_CAND) {
+    uint64_t b1 = ~0ull;                                        // above every entry: ids are below 2^24
+    while (b1 - b0 > 1) {
+      const uint64_t mid = b0 + ((b1 - b0) >> 1);
+      int q = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) q += o[i] >= mid ? 1 : 0;
+      q = block_count<NT>(q, cnt);
+      if (q >= k) {
+        b0 = mid;
+        if (q <= TOP_CAND) break;
+      } else {
+        b1 = mid;
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (o[i] >= b0) cand[atomicAdd(&n_cand, 1)] = o[i];
+  __syncthreads();
+  rank_out<NT>(cand, n_cand, k, [&](int rank, uint64_t q) {
+    index[r * k + rank] = entry_id(q);
+    values[r * k + rank] = D::put(key_value((uint32_t)(q >> 32)));
+  });
+  if (threadIdx.x < 64) {
+    double m = -FLT_MAX, s = 0;
+    for (int i = threadIdx.x; i < n_chunk; i += 64) m = fmax(m, parts[r * n_chunk + i].m);
+    m = wave_max_d(m);
+    for (int i = threadIdx.x; i < n_chunk; i += 64) s += parts[r * n_chunk + i].s * exp((parts[r * n_chunk + i].m - m) * inv_temp);
+    s = wave_sum_d(s);
+    if (threadIdx.x == 0) lse[r] = (float)(m * inv_temp + log(s));
+  }
+}
+
+// A chunk holds at most 16 vectors a thread, and not less than 16 k elements (or its list would be most of it).
+static int top_chunks(int rows, int V, int k, int dtype) {
+  const int n = row_chunks(rows, V, 256 * 16 * (16 / row_size(dtype)), 16 * k > 2048 ? 16 * k : 2048);
+  return n * k <= TOP_MAX_LIST ? n : row_chunks(512, V, 256 * 16 * (16 / row_size(dtype)), 1);
+}
+
+extern "C" int64_t nast_top_logits_workspace_bytes(int rows, int V, int k, int dtype) {
+  if (rows < 1 || V < 1 || k < 1 || !row_dtype_ok(dtype)) return 0;
+  const int64_t n = top_chunks(rows, V, k, dtype);
+  return n > 1 ? rows * n * (k * (int64_t)sizeof(uint64_t) + (int64_t)sizeof(MaxSumD)) : 0;
+}
+
+template <class D, int NV>
+static void top_launch(const void* x, nast_rows xr, void* values, int64_t* index, float* lse, uint64_t* lists, MaxSumD* parts, int rows,
+                       int V, int k, int chunk, int n, double temp, hipStream_t s) {
+  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NV>), dim3(rows * n), dim3(256), 0, s, (const typename D::store*)x, xr,
+                     (typename D::store*)values, index, lse, lists, parts, V, k, chunk, n, 1.0 / temp, exp_scale(temp));
+  if (n > 1 && n * k <= 4096)
+    hipLaunchKernelGGL((nast_top_join_kernel<D, 256>), dim3(rows), dim3(256), 0, s, lists, parts, (typename D::store*)values, index, lse, k, n,
+                       1.0 / temp);
+  else if (n > 1)
+    hipLaunchKernelGGL((nast_top_join_kernel<D, 1024>), dim3(rows), dim3(1024), 0, s, lists, parts, (typename D::store*)values, index, lse, k,
+                       n, 1.0 / temp);
+}
 
 extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* values, int64_t* index, float* lse, int rows, int V,
                                int k, double temp, void* workspace, void* stream) {
   NAST_REQUIRE(row_dtype_ok(dtype), "nast_top_logits: unknown dtype %d", dtype);
-  NAST_REQUIRE(rows >= 0 && V >= 1 && V < (1 << 24), "nast_top_logits: bad sizes rows=%d V=%d", rows, V);
+  NAST_REQUIRE(rows >= 0 && V >= 1 && V <= (1 << 20), "nast_top_logits: bad sizes rows=%d V=%d", rows, V);
   NAST_REQUIRE(k >= 1 && k <= TOP_MAX_K && k <= V, "nast_top_logits: k=%d must lie in [1, %d] and not exceed V=%d", k, TOP_MAX_K, V);
   NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_top_logits: temperature must be > 0 and finite");
   if (rows == 0) return NAST_OK;
-  NAST_REQUIRE(rows < (1 << 24), "nast_top_logits: too many rows (%d)", rows);
-  NAST_REQUIRE(x && values && index && lse, "nast_top_logits: NULL pointer");
+  const int n = top_chunks(rows, V, k, dtype), chunk = (V + n - 1) / n;
+  NAST_REQUIRE((int64_t)rows * n < (1 << 22), "nast_top_logits: too many rows (%d)", rows);
+  NAST_REQUIRE(x && values && index && lse && (n == 1 || workspace), "nast_top_logits: NULL pointer");
   NAST_REQUIRE(row_aligned(x, dtype) && row_aligned(values, dtype), "nast_top_logits: misaligned pointer");
-  nast_prof_before(2, (hipStream_t)stream);
-  NAST_ROW_DTYPE(dtype, hipLaunchKernelGGL((nast_top_logits_kernel<D>), dim3(rows), dim3(256), 0, (hipStream_t)stream,
-                                           (const typename D::store*)x, xr, (typename D::store*)values, index, lse, V, k, 1.0 / temp,
-                                           exp_scale(temp)));
-  nast_prof_after(2, (hipStream_t)stream, (double)row_size(dtype) * rows * (double)V);
+  hipStream_t s = (hipStream_t)stream;
+  uint64_t* lists = (uint64_t*)workspace;
+  MaxSumD* parts = n > 1 ? (MaxSumD*)(lists + (int64_t)rows * n * k) : nullptr;
+  const int nv = (chunk / (16 / row_size(dtype)) + 255) / 256;      // vectors a thread
+  nast_prof_before(2, s);
+#define NAST_TOP(NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, chunk, n, temp, s)))
+  if (nv <= 2) NAST_TOP(2);
+  else if (nv <= 4) NAST_TOP(4);
+  else if (nv <= 8) NAST_TOP(8);
+  else if (nv <= 12) NAST_TOP(12);
+  else NAST_TOP(16);
+#undef NAST_TOP
+  nast_prof_after(2, s, (double)row_size(dtype) * rows * (double)V);
   NAST_CHECK_LAUNCH("nast_top_logits");
   return NAST_OK;
 }
@@ -198,42 +470,63 @@ __device__ void distill_finish(int64_t r, MaxSumD rest, const typename D::store*
 
 // One workgroup per chunk of a row: (max, exponential sum) of the tokens that no used slot names.  The named ones are marked in LDS,
 // one bit per element, and left out of both: their terms are added in double at the end, and q_r is a sum and no difference.
+// Rows are taken from the last to the first: the backward pass, from the first to the last, then begins with what this pass has
+// left in the last-level cache (256 MB), and this pass with what the product that made the logits has left there.
 template <class D, bool SPLIT>
 __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                                    const void* __restrict__ t, int t_dtype,
                                                                    const int64_t* __restrict__ idx, int K,
                                                                    const float* __restrict__ lse_t, float* __restrict__ loss,
                                                                    DistillStats* __restrict__ stats, MaxSumD* __restrict__ parts, int V,
-                                                                   int chunk, int n_chunk, double it, ExpScale c) {
-  __shared__ uint32_t bits[DISTILL_CHUNK / 32 + 1];
+                                                                   int chunk, int n_chunk, double it, float c) {
+  constexpr int U = 4;
+  __shared__ uint32_t bits[DISTILL_CHUNK / 32 + 2];            // bit EPV + i: element body + i
   __shared__ double red[8];
   __shared__ uint32_t ids[DISTILL_MAX_K];
-  const int64_t r = blockIdx.x / n_chunk;
-  const int lo = (int)(blockIdx.x % n_chunk) * chunk, hi = min(V, lo + chunk);
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int64_t r = block / n_chunk;
+  const int lo = (int)(block % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
-  const RowSlots<D> rs(p, lo, hi);
-  for (int w = threadIdx.x; w < (hi - rs.first + 31) / 32; w += 256) bits[w] = 0;
+  const RowSpan16<D> rs(p, lo, hi);
+  const int bit0 = rs.body - D::EPV;
+  for (int w = threadIdx.x; w < (hi - bit0 + 31) / 32; w += 256) bits[w] = 0;
   __syncthreads();
   for (int j = threadIdx.x; j < K; j += 256) {
     const int64_t id = idx[r * K + j];
     if (id >= lo && id < hi && slot_used(id, teacher_logit(t, t_dtype, r * K + j), V))
-      atomicOr(&bits[(id - rs.first) >> 5], 1u << ((id - rs.first) & 31));
+      atomicOr(&bits[(id - bit0) >> 5], 1u << ((id - bit0) & 31));
   }
   __syncthreads();
   MaxSum a{-FLT_MAX, 0.f};
-  for (int s = threadIdx.x; s < rs.n; s += 256) {
-    RowVec<D> v = rs.load(p, s);
-    const uint32_t named = bits[s * D::EPV >> 5] >> (s * D::EPV & 31);
-    if (named & ((1u << D::EPV) - 1)) {
+  for (int base = threadIdx.x; base < rs.n; base += 256 * U) {
+    RowVec<D> v[U];
 #pragma unroll
-      for (int i = 0; i < D::EPV; ++i)
-        if (named >> i & 1) v.e[i] = D::put(-INFINITY);
+    for (int u = 0; u < U; ++u) {
+      const int s = base + 256 * u;
+      if (s < rs.n) {
+        v[u] = rs.load(p, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(-INFINITY);
+      }
     }
-    fold<D>(a, v, c);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int at = (base + 256 * u + 1) * D::EPV;
+      const uint32_t named = base + 256 * u < rs.n ? bits[at >> 5] >> (at & 31) & ((1u << D::EPV) - 1) : 0;
+      if (named) {
+#pragma unroll
+        for (int i = 0; i < D::EPV; ++i)
+          if (named >> i & 1) v[u].e[i] = D::put(-INFINITY);
+      }
+    }
+    fold<D, U>(a, v, c);
   }
+  const int e = rs.edge(threadIdx.x);
+  if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(p[e]), c);
   const MaxSumD rest = block_max_sum<256>(a, c, red);
   if (SPLIT) {
-    if (threadIdx.x == 0) parts[blockIdx.x] = rest;
+    if (threadIdx.x == 0) parts[block] = rest;
   } else if (threadIdx.x < 64) {
     distill_finish<D>(r, rest, p, t, t_dtype, idx, K, lse_t, loss, stats, V, it, ids);
   }
@@ -268,7 +561,8 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
                                                                    const int64_t* __restrict__ idx, int K,
                                                                    const DistillStats* __restrict__ stats,
                                                                    typename D::store* __restrict__ gx, nast_rows gxr, int V, int chunk,
-                                                                   int n_chunk, double it, ExpScale c) {
+                                                                   int n_chunk, double it, float c) {
+  constexpr int U = 4;
   __shared__ uint32_t ids[DISTILL_MAX_K];
   __shared__ float ts[DISTILL_MAX_K];
   const int64_t r = blockIdx.x / n_chunk;
@@ -291,31 +585,22 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
   }
   // a factor of 0 (a row without a list, a row of no weight) writes zeros whatever the logits hold
   const float F = gr == 0 ? 0.f : (float)(gr * st.coef), m = (float)st.m_rest;
-  const RowSlots<D> rs(o, lo, hi);
-  const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
-  for (int s = threadIdx.x; s < rs.n; s += 256) {
-    RowVec<D> v;
-    if (same) {
-      v = rs.load(p, s);
-    } else {
+  const RowSpan16<D> rs(o, lo, hi);
+  for (int base = threadIdx.x; base < rs.n; base += 256 * U) {
+    RowVec<D> v[U];
 #pragma unroll
-      for (int i = 0; i < D::EPV; ++i) {
-        const int e = rs.elem(s) + i;
-        v.e[i] = e >= lo && e < hi ? p[e] : D::put(0.f);
-      }
-    }
+    for (int u = 0; u < U; ++u)
+      if (base + 256 * u < rs.n) v[u] = load16<D>(p + rs.elem(base + 256 * u));
 #pragma unroll
-    for (int i = 0; i < D::EPV; ++i) v.e[i] = D::put(F == 0.f ? 0.f : exp_t(D::get(v.e[i]) - m, c) * F);
-    if (rs.whole(s)) {
-      *reinterpret_cast<uint4*>(o + rs.elem(s)) = v.raw;
-    } else {
+    for (int u = 0; u < U; ++u) {
+      if (base + 256 * u >= rs.n) break;
 #pragma unroll
-      for (int i = 0; i < D::EPV; ++i) {
-        const int e = rs.elem(s) + i;
-        if (e >= lo && e < hi) o[e] = v.e[i];
-      }
+      for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(F == 0.f ? 0.f : exp_t(D::get(v[u].e[i]) - m, c) * F);
+      *reinterpret_cast<uint4*>(o + rs.elem(base + 256 * u)) = v[u].raw;
     }
   }
+  const int e = rs.edge(threadIdx.x);
+  if (e >= 0) o[e] = D::put(F == 0.f ? 0.f : exp_t(D::get(p[e]) - m, c) * F);
   __syncthreads();
   if (id == DISTILL_NO_ID) return;
   double pj = 0;
@@ -355,7 +640,7 @@ extern "C" int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, cons
   hipStream_t s = (hipStream_t)stream;
   DistillStats* st = (DistillStats*)stats;
   MaxSumD* parts = (MaxSumD*)workspace;
-  const ExpScale c = exp_scale(temp);
+  const float c = exp_scale(temp);
   nast_prof_before(2, s);
   NAST_ROW_DTYPE(dtype, {
     const typename D::store* xp = (const typename D::store*)x;

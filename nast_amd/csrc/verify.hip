@@ -26,7 +26,7 @@ struct VerifyArgs {
   int64_t *out, *accepted;
   int B, N, V, chunk, n_chunk;
   double it;                      // 1 / T
-  ExpScale c;
+  float c;
   MaxSumD* parts;                 // [B * (2 N + 1)][n_chunk]: target rows first, then draft rows
   struct VerifyBest* best;        // [B][n_chunk]
 };
@@ -72,9 +72,7 @@ __global__ __launch_bounds__(256) void nast_verify_lse_kernel(VerifyArgs A) {
   const int len = draft_length(A, b);
   if (is_target ? i > len : i >= len) return;
   const typename D::store* p = is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i);
-  const RowSlots<D> rs(p, lo, hi);
-  MaxSum a{-FLT_MAX, 0.f};
-  for (int s = threadIdx.x; s < rs.n; s += 256) fold<D>(a, rs.load(p, s), A.c);
+  const MaxSum a = span_max_sum<D, 256>(p, lo, hi, A.c);
   const MaxSumD t = block_max_sum<256>(a, A.c, red);
   if (threadIdx.x == 0) A.parts[blockIdx.x] = t;
 }
