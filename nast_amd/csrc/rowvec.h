@@ -7,39 +7,65 @@
 
 // One struct per storage type: EPV elements in 16 bytes, their conversion to fp32 (exact) and back (to nearest even); the low
 // KEY_ZEROS bits of an fp32 mantissa that no value of the type uses.
+// Vectors are kept as four words: as eight halves the compiler gives each a register.
 struct RowF32 {
   using store = float;
   static constexpr int EPV = 4, KEY_ZEROS = 0;
   static __device__ __forceinline__ float get(store v) { return v; }
   static __device__ __forceinline__ store put(float v) { return v; }
+  static __device__ __forceinline__ float unpack(uint32_t w, int) { return __builtin_bit_cast(float, w); }
+  static __device__ __forceinline__ uint32_t pack(const float* f) { return __builtin_bit_cast(uint32_t, f[0]); }
 };
 struct RowBF16 {
   using store = __bf16;
+  using pair = __bf16 __attribute__((ext_vector_type(2)));
   static constexpr int EPV = 8, KEY_ZEROS = 16;
   static __device__ __forceinline__ float get(store v) { return (float)v; }
   static __device__ __forceinline__ store put(float v) { return (store)v; }
+  static __device__ __forceinline__ float unpack(uint32_t w, int half) { return __builtin_bit_cast(float, half ? w & 0xffff0000u : w << 16); }
+  static __device__ __forceinline__ uint32_t pack(const float* f) { return __builtin_bit_cast(uint32_t, pair{(store)f[0], (store)f[1]}); }
 };
 struct RowF16 {
   using store = _Float16;
+  using pair = _Float16 __attribute__((ext_vector_type(2)));
   static constexpr int EPV = 8, KEY_ZEROS = 13;
   static __device__ __forceinline__ float get(store v) { return (float)v; }
   static __device__ __forceinline__ store put(float v) { return (store)v; }
+  static __device__ __forceinline__ float unpack(uint32_t w, int half) { return (float)__builtin_bit_cast(pair, w)[half]; }
+  static __device__ __forceinline__ uint32_t pack(const float* f) { return __builtin_bit_cast(uint32_t, pair{(store)f[0], (store)f[1]}); }
 };
 
 template <class D>
-union RowVec {
-  uint4 raw;
-  typename D::store e[D::EPV];
+struct RowVec {
+  static constexpr int PER = D::EPV / 4;   // elements a word
+  uint32_t w[4];
+  __device__ __forceinline__ float get(int i) const { return D::unpack(w[i / PER], i % PER); }
+  __device__ __forceinline__ void put(const float (&f)[D::EPV]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = D::pack(f + i * PER);
+  }
 };
-
+template <class D>
+__device__ __forceinline__ RowVec<D> vec_of(float f) {   // one value in every element
+  const float two[2] = {f, f};
+  const uint32_t w = D::pack(two);
+  return {{w, w, w, w}};
+}
+template <class D>
+__device__ __forceinline__ RowVec<D> vec_load(const typename D::store* p) {   // p 16-byte aligned
+  const uint4 q = *reinterpret_cast<const uint4*>(p);
+  return {{q.x, q.y, q.z, q.w}};
+}
+template <class D>
+__device__ __forceinline__ void vec_store(typename D::store* p, const RowVec<D>& v) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+}
 // 16 bytes from any element: global_load_dwordx4 takes any alignment on this target
 typedef uint32_t raw16_any __attribute__((ext_vector_type(4), aligned(2)));
 template <class D>
-__device__ __forceinline__ RowVec<D> load16(const typename D::store* p) {
+__device__ __forceinline__ RowVec<D> vec_load_any(const typename D::store* p) {
   const raw16_any q = *reinterpret_cast<const raw16_any*>(p);
-  RowVec<D> v;
-  v.raw = make_uint4(q.x, q.y, q.z, q.w);
-  return v;
+  return {{q.x, q.y, q.z, q.w}};
 }
 
 // Elements [lo, hi) of a row: a body of whole 16-byte aligned vectors, slot s at element body + s * EPV, and at most EPV - 1 elements
@@ -55,9 +81,7 @@ struct RowSpan16 {
   }
   __device__ __forceinline__ int elem(int s) const { return body + s * D::EPV; }
   __device__ __forceinline__ RowVec<D> load(const typename D::store* p, int s) const {
-    RowVec<D> v;
-    v.raw = *reinterpret_cast<const uint4*>(p + body + s * D::EPV);
-    return v;
+    return vec_load<D>(p + body + s * D::EPV);
   }
   // the element thread t has to look after besides its slots, or -1
   __device__ __forceinline__ int edge(int t) const {
@@ -84,7 +108,7 @@ __device__ __forceinline__ void fold(MaxSum& a, const RowVec<D> (&v)[U], float c
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < D::EPV; ++i) top = fmaxf(top, D::get(v[u].e[i]));
+    for (int i = 0; i < D::EPV; ++i) top = fmaxf(top, v[u].get(i));
   if (top > a.m) {
     a.s *= exp_t(a.m - top, c);
     a.m = top;
@@ -93,7 +117,7 @@ __device__ __forceinline__ void fold(MaxSum& a, const RowVec<D> (&v)[U], float c
   for (int u = 0; u < U; ++u) {
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < D::EPV; ++i) s += exp_t(D::get(v[u].e[i]) - a.m, c);
+    for (int i = 0; i < D::EPV; ++i) s += exp_t(v[u].get(i) - a.m, c);
     a.s += s;
   }
 }
@@ -115,12 +139,8 @@ __device__ __forceinline__ MaxSum span_max_sum(const typename D::store* p, int l
     RowVec<D> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (base + NT * u < rs.n) {
-        v[u] = rs.load(p, base + NT * u);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(-INFINITY);
-      }
+      v[u] = vec_of<D>(-INFINITY);
+      if (base + NT * u < rs.n) v[u] = rs.load(p, base + NT * u);
     }
     fold<D, U>(a, v, c);
   }

@@ -52,7 +52,7 @@ __device__ __forceinline__ int block_count(int n, int* cnt) {   // n <= 2^16 a t
 // values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the
 // registers, and equal elements are taken in the order of their ids.
 template <class D, int NV>
-__global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
+__global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
                                                              float* __restrict__ lse, uint64_t* __restrict__ lists,
                                                              MaxSumD* __restrict__ parts, int V, int k, int chunk, int n_chunk,
@@ -71,12 +71,8 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
   RowVec<D> v[NV];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i * 256 < rs.n) {
-      if (i * 256 + tid < rs.n) v[i] = rs.load(p, i * 256 + tid);
-      else
-#pragma unroll
-        for (int j = 0; j < D::EPV; ++j) v[i].e[j] = D::put(-INFINITY);
-    }
+    v[i] = vec_of<D>(-INFINITY);
+    if (i * 256 + tid < rs.n) v[i] = rs.load(p, i * 256 + tid);
   }
   const int ee = rs.edge(tid);
   const float ef = ee >= 0 ? D::get(p[ee]) : -INFINITY;
@@ -89,12 +85,15 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     vm[i] = -INFINITY;
-    if (i * 256 < rs.n) {
 #pragma unroll
-      for (int j = 0; j < D::EPV; ++j) vm[i] = fmaxf(vm[i], D::get(v[i].e[j]));
-      g[i % G] = fmaxf(g[i % G], vm[i]);
-    }
+    for (int j = 0; j < D::EPV; ++j) vm[i] = fmaxf(vm[i], v[i].get(j));
+    g[i % G] = fmaxf(g[i % G], vm[i]);
+    __builtin_amdgcn_sched_barrier(0);
   }
+  // from here the vectors are unpacked once more for the sum: the compiler must not keep what it has unpacked (half the kernel's
+  // occupancy at 16-bit types)
+#pragma unroll
+  for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(v[i].w[0]), "+v"(v[i].w[1]), "+v"(v[i].w[2]), "+v"(v[i].w[3]));
   const int groups = G > 1 && k > 64 ? G : 1;
   if (groups > 1) {
 #pragma unroll
@@ -153,7 +152,7 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
     hits &= hits - 1;
     const RowVec<D> w = rs.load(p, s);
     for (int j = 0; j < D::EPV; ++j) {
-      const float f = D::get(w.e[j]);
+      const float f = w.get(j);
       if (f >= thr) {
         const int at = atomicAdd(&n_cand, 1);
         if (at < TOP_CAND) cand[at] = top_entry(f, rs.elem(s) + j);
@@ -168,9 +167,10 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
     if (i * 256 < rs.n) {
       float t = 0.f;
 #pragma unroll
-      for (int j = 0; j < D::EPV; ++j) t += exp_t(D::get(v[i].e[j]) - m, c);
+      for (int j = 0; j < D::EPV; ++j) t += exp_t(v[i].get(j) - m, c);
       sum += t;
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
   const double ws = wave_sum_d((double)sum);
   if (lane == 0) red[tid >> 6] = ws;
@@ -178,15 +178,15 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
   const double s = (red[0] + red[1]) + (red[2] + red[3]);
   int n = n_cand;
 
-  if (s != s || n > TOP_CAND) {
+  if (s != s || n > TOP_CAND) {                                 // (from memory again: a copy in registers would cost every row its place)
     constexpr int SHIFT = D::KEY_ZEROS;
     auto count = [&](uint64_t at_least) {                       // elements with key >> SHIFT at or above
       int q = ee >= 0 && (order_key(ef) >> SHIFT) >= at_least ? 1 : 0;
+      for (int s = tid; s < rs.n; s += 256) {
+        const RowVec<D> w = rs.load(p, s);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i * 256 + tid < rs.n)
-#pragma unroll
-          for (int j = 0; j < D::EPV; ++j) q += (order_key(D::get(v[i].e[j])) >> SHIFT) >= at_least ? 1 : 0;
+        for (int j = 0; j < D::EPV; ++j) q += (order_key(w.get(j)) >> SHIFT) >= at_least ? 1 : 0;
+      }
       return block_count<256>(q, cnt);
     };
     uint64_t b0 = 0, b1 = 1ull << (32 - SHIFT);
@@ -200,32 +200,27 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
     __syncthreads();
     int before = 0;
     // pieces of ascending ids: head, the vectors one row of slots after the other, tail
-    for (int piece = -1; piece <= NV; ++piece) {
-      if (piece >= 0 && piece < NV && piece * 256 >= rs.n) continue;
-      uint64_t mine[D::EPV];
-      int same = 0;
-      uint32_t is_same = 0, is_more = 0;
-      if (piece == -1 || piece == NV) {
+    const int pieces = (rs.n + 255) / 256;
+    for (int piece = -1; piece <= pieces; ++piece) {
+      const int s = piece * 256 + tid;
+      uint32_t same = 0, more = 0;
+      RowVec<D> w = vec_of<D>(ef);                              // an edge element stands first
+      if (piece == -1 || piece == pieces) {
         const bool here = ee >= 0 && (piece == -1) == (ee < rs.body);
         const uint32_t key = order_key(ef) >> SHIFT;
-        mine[0] = top_entry(ef, ee);
-        is_same = here && key == b0 ? 1 : 0;
-        is_more = here && key > b0 ? 1 : 0;
-      } else {
+        same = here && key == b0 ? 1 : 0;
+        more = here && key > b0 ? 1 : 0;
+      } else if (s < rs.n) {
+        w = rs.load(p, s);
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (i == piece && i * 256 + tid < rs.n)
-#pragma unroll
-            for (int j = 0; j < D::EPV; ++j) {
-              const float f = D::get(v[i].e[j]);
-              const uint32_t key = order_key(f) >> SHIFT;
-              mine[j] = top_entry(f, rs.elem(i * 256 + tid) + j);
-              is_same |= (key == b0 ? 1u : 0u) << j;
-              is_more |= (key > b0 ? 1u : 0u) << j;
-            }
+        for (int j = 0; j < D::EPV; ++j) {
+          const uint32_t key = order_key(w.get(j)) >> SHIFT;
+          same |= (key == b0 ? 1u : 0u) << j;
+          more |= (key > b0 ? 1u : 0u) << j;
+        }
       }
-      same = __popc(is_same);
-      int scan = same;                                          // inclusive over the wavefront
+      int scan = __popc(same);                                  // inclusive over the wavefront
+      const int own = scan;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int q = __shfl_up(scan, o, 64);
@@ -234,7 +229,7 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
       __syncthreads();
       if (lane == 63) cnt[tid >> 6] = scan;
       __syncthreads();
-      int place = before + scan - same;
+      int place = before + scan - own;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i < tid >> 6) place += cnt[i];
@@ -242,8 +237,9 @@ __global__ __launch_bounds__(256) void nast_top_chunk_kernel(const typename D::s
       }
 #pragma unroll
       for (int j = 0; j < D::EPV; ++j) {
-        const bool eq = is_same >> j & 1;
-        if ((eq && place < need) || (is_more >> j & 1)) cand[atomicAdd(&n_cand, 1)] = mine[j];
+        const bool eq = same >> j & 1;
+        if ((eq && place < need) || (more >> j & 1))
+          cand[atomicAdd(&n_cand, 1)] = top_entry(w.get(j), piece == -1 || piece == pieces ? ee : rs.elem(s) + j);
         place += eq ? 1 : 0;
       }
     }
@@ -502,13 +498,8 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
     RowVec<D> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int s = base + 256 * u;
-      if (s < rs.n) {
-        v[u] = rs.load(p, s);
-      } else {
-#pragma unroll
-        for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(-INFINITY);
-      }
+      v[u] = vec_of<D>(-INFINITY);
+      if (base + 256 * u < rs.n) v[u] = rs.load(p, base + 256 * u);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -516,8 +507,12 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
       const uint32_t named = base + 256 * u < rs.n ? bits[at >> 5] >> (at & 31) & ((1u << D::EPV) - 1) : 0;
       if (named) {
 #pragma unroll
-        for (int i = 0; i < D::EPV; ++i)
-          if (named >> i & 1) v[u].e[i] = D::put(-INFINITY);
+        for (int i = 0; i < 4; ++i) {
+          float f[2];
+#pragma unroll
+          for (int j = 0; j < RowVec<D>::PER; ++j) f[j] = named >> (i * RowVec<D>::PER + j) & 1 ? -INFINITY : D::unpack(v[u].w[i], j);
+          v[u].w[i] = D::pack(f);
+        }
       }
     }
     fold<D, U>(a, v, c);
@@ -590,13 +585,15 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
     RowVec<D> v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (base + 256 * u < rs.n) v[u] = load16<D>(p + rs.elem(base + 256 * u));
+      if (base + 256 * u < rs.n) v[u] = vec_load_any<D>(p + rs.elem(base + 256 * u));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (base + 256 * u >= rs.n) break;
+      float f[D::EPV];
 #pragma unroll
-      for (int i = 0; i < D::EPV; ++i) v[u].e[i] = D::put(F == 0.f ? 0.f : exp_t(D::get(v[u].e[i]) - m, c) * F);
-      *reinterpret_cast<uint4*>(o + rs.elem(base + 256 * u)) = v[u].raw;
+      for (int i = 0; i < D::EPV; ++i) f[i] = F == 0.f ? 0.f : exp_t(v[u].get(i) - m, c) * F;
+      v[u].put(f);
+      vec_store<D>(o + rs.elem(base + 256 * u), v[u]);
     }
   }
   const int e = rs.edge(threadIdx.x);
