@@ -134,18 +134,21 @@ template <class D, int NT>
 __device__ __forceinline__ MaxSum span_max_sum(const typename D::store* p, int lo, int hi, float c) {
   constexpr int U = 4;
   const RowSpan16<D> rs(p, lo, hi);
+  const int e = rs.edge(threadIdx.x);
+  const typename D::store edge = p[e >= 0 ? e : lo];
   MaxSum a{-FLT_MAX, 0.f};
-  for (int base = threadIdx.x; base < rs.n; base += NT * U) {
+  int base = threadIdx.x;
+  for (; base + NT * (U - 1) < rs.n; base += NT * U) {     // (no branch around a load: the compiler would wait for each before the next)
     RowVec<D> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = vec_of<D>(-INFINITY);
-      if (base + NT * u < rs.n) v[u] = rs.load(p, base + NT * u);
-    }
+    for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + NT * u);
     fold<D, U>(a, v, c);
   }
-  const int e = rs.edge(threadIdx.x);
-  if (e >= 0) fold_one(a, D::get(p[e]), c);
+  for (; base < rs.n; base += NT) {
+    const RowVec<D> v[1] = {rs.load(p, base)};
+    fold<D, 1>(a, v, c);
+  }
+  if (e >= 0) fold_one(a, D::get(edge), c);
   return a;
 }
 
@@ -181,6 +184,15 @@ __device__ __forceinline__ MaxSumD block_max_sum(MaxSum a, float c, double* red)
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) s += red[2 * i + 1] * (double)exp_t((float)(red[2 * i] - m), c);
   return {m, s};
+}
+
+__device__ __forceinline__ int lanes_below(uint64_t mask) {    // how many bits of the mask lie below this lane's
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+// what a lane has written to LDS is there for the other lanes of its wavefront
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // Key whose unsigned order is the order of the values: -0 equals +0, NaN (any) above +inf.

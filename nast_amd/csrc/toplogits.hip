@@ -11,7 +11,8 @@
 // top logits
 // ---------------------------------------------------------------------------------------------
 #define TOP_MAX_K 256
-#define TOP_CAND 512              // candidates a workgroup ranks
+#define TOP_MAX_V (1 << 20)
+#define TOP_WAVE 128              // candidates a wavefront keeps
 #define TOP_MAX_LIST 16384        // entries the join of a row's chunks takes
 
 // Elements are ordered by value, ties to the lower id: entry = key << 32 | ~id is one 64-bit number per element, no two alike, 0 is
@@ -19,13 +20,28 @@
 __device__ __forceinline__ uint64_t top_entry(float f, int e) { return ((uint64_t)order_key(f) << 32) | (uint32_t)~e; }
 __device__ __forceinline__ int entry_id(uint64_t o) { return (int)~(uint32_t)o; }
 
-// Each of n <= TOP_CAND distinct entries in LDS is written at its rank among them, up to rank k.
-template <int NT, class F>
-__device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, F&& out) {
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const uint64_t o = cand[i];
+// Distinct entries in LDS, n[g] of them at cand + g * STRIDE: each goes to out(rank among all, entry) where the rank is below k.  A rank
+// is a count of larger entries.
+template <int NT, int GROUPS, int STRIDE, class F>
+__device__ __forceinline__ void rank_out(const uint64_t* cand, const int (&n)[GROUPS], int k, F&& out) {
+  int all = 0;
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) all += n[g];
+  for (int i = threadIdx.x; i < all; i += NT) {
+    int at = i, g = 0;
+#pragma unroll
+    for (int h = 0; h < GROUPS - 1; ++h)
+      if (g == h && at >= n[h]) {
+        at -= n[h];
+        ++g;
+      }
+    const uint64_t o = cand[g * STRIDE + at];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand[j] > o ? 1 : 0;
+#pragma unroll
+    for (int h = 0; h < GROUPS; ++h) {
+#pragma unroll 4
+      for (int j = 0; j < n[h]; ++j) rank += cand[h * STRIDE + j] > o ? 1 : 0;
+    }
     if (rank < k) out(rank, o);
   }
 }
@@ -42,41 +58,91 @@ __device__ __forceinline__ int block_count(int n, int* cnt) {   // n <= 2^16 a t
   return t;
 }
 
+// By one wavefront: bound[0] = a value that at least kk of the 64 * N group maxima reach (and, where one is found, not more than
+// 5/4 kk + 8), bound[1] = the largest.  Bisection on the upper half of the order key.
+template <int N>
+__device__ __forceinline__ void group_bound(const float* gmax, int kk, float* bound) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY, least = INFINITY;
+  uint32_t key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = gmax[i * 64 + lane];
+    m = fmaxf(m, f);
+    least = fminf(least, f);
+    key[i] = order_key(f) >> 16;
+  }
+  m = wave_max(m);
+  least = -wave_max(-least);
+  uint32_t b0 = order_key(least) >> 16, b1 = (order_key(m) >> 16) + 1;
+  while (b1 - b0 > 1) {
+    const uint32_t mid = (b0 + b1) >> 1;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= mid));
+    if (n >= kk) {
+      b0 = mid;
+      if (n <= kk + kk / 4 + 8) break;
+    } else {
+      b1 = mid;
+    }
+  }
+  b0 <<= 16;
+  if (lane == 0) {
+    bound[0] = b0 < 0x00800000u ? -INFINITY : key_value(b0);   // (keys below that of -inf are of no number)
+    bound[1] = fmaxf(m, -FLT_MAX);
+  }
+}
+
+// What a chunk leaves beside its list: maximum and exponential sum, and a bound that at least k of its elements reach (-inf: unknown).
+struct TopPart {
+  double m, s;
+  float bound;
+};
+
 // One workgroup per chunk of a row, the chunk in registers: NV vectors a thread (and an edge element), read from memory once.
 //
 // The k-th largest of the maxima of disjoint groups of elements is a lower bound of the k-th largest element.  Each thread keeps the
-// maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and every
-// wavefront finds a bound among them by bisection on the upper half of the order key, content with up to k + k/4 + 8 groups at
-// or above it.  Vectors whose maximum reaches the bound are looked through again; what is found there (a little more than k
-// elements where they lie at random) is ranked by counting.  Where more than TOP_CAND elements reach the bound (many equal
-// values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the
+// maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and one
+// wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to LDS, each wavefront's to a place of
+// its own, where its lanes look at their elements one by one; what reaches the bound (a little more than k elements where they lie at
+// random) is ranked by counting.  Where more than TOP_WAVE elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the
 // registers, and equal elements are taken in the order of their ids.
 template <class D, int NV>
 __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
                                                              float* __restrict__ lse, uint64_t* __restrict__ lists,
-                                                             MaxSumD* __restrict__ parts, int V, int k, int chunk, int n_chunk,
+                                                             TopPart* __restrict__ parts, int V, int k, int len, int chunk, int n_chunk,
                                                              double inv_temp, float c) {
   constexpr int G = NV >= 4 ? 4 : 1;
   __shared__ float gmax[256 * G];
-  __shared__ uint64_t cand[TOP_CAND];
+  __shared__ uint64_t cand[4 * TOP_WAVE];
+  __shared__ uint4 vec_data[4 * TOP_WAVE];
+  __shared__ int vec_slot[4 * TOP_WAVE];
   __shared__ double red[4];
   __shared__ int cnt[4];
+  __shared__ float bound[2];
   __shared__ int n_cand;
   const int64_t r = blockIdx.x / n_chunk;
   const int tid = threadIdx.x, lane = tid & 63, lo = (int)(blockIdx.x % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
   const RowSpan16<D> rs(p, lo, hi);
   const int kk = min(k, hi - lo);
-  RowVec<D> v[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    v[i] = vec_of<D>(-INFINITY);
-    if (i * 256 + tid < rs.n) v[i] = rs.load(p, i * 256 + tid);
-  }
   const int ee = rs.edge(tid);
-  const float ef = ee >= 0 ? D::get(p[ee]) : -INFINITY;
-  if (tid == 0) n_cand = 0;
+  const typename D::store edge = p[ee >= 0 ? ee : lo];
+  RowVec<D> v[NV];
+  // (no branch around a single load: the compiler would wait for each before the next)
+  if (rs.n > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = rs.load(p, min(i * 256 + tid, rs.n - 1));
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = vec_of<D>(-INFINITY);
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i + 1) * 256 > rs.n && i * 256 + tid >= rs.n) v[i] = vec_of<D>(-INFINITY);
+  const float ef = ee >= 0 ? D::get(edge) : -INFINITY;
 
   float vm[NV], g[G];
 #pragma unroll
@@ -105,62 +171,30 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   }
   __syncthreads();
 
-  // the bound, by every wavefront for itself
-  float m = -INFINITY, least = INFINITY, thr;
-  uint32_t gk[4 * G];
-#pragma unroll
-  for (int i = 0; i < 4 * G; ++i) {
-    gk[i] = 0;
-    if (i < 4 * groups) {
-      const float f = gmax[i * 64 + lane];
-      m = fmaxf(m, f);
-      least = fminf(least, f);
-      gk[i] = order_key(f) >> 16;
-    }
+  if (tid < 64) {
+    if (groups > 1) group_bound<4 * G>(gmax, kk, bound);
+    else group_bound<4>(gmax, kk, bound);
   }
-  m = wave_max(m);
-  least = -wave_max(-least);
-  {
-    uint32_t b0 = order_key(least) >> 16, b1 = (order_key(m) >> 16) + 1;
-    while (b1 - b0 > 1) {
-      const uint32_t mid = (b0 + b1) >> 1;
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < 4 * G; ++i)
-        if (i < 4 * groups) n += __popcll(__ballot(gk[i] >= mid));
-      if (n >= kk) {
-        b0 = mid;
-        if (n <= kk + kk / 4 + 8) break;
-      } else {
-        b1 = mid;
-      }
-    }
-    b0 <<= 16;
-    thr = b0 < 0x00800000u ? -INFINITY : key_value(b0);
-  }
+  __syncthreads();
+  const float thr = bound[0], m = bound[1];
 
-  if (ef >= thr && ee >= 0) {
-    const int at = atomicAdd(&n_cand, 1);
-    if (at < TOP_CAND) cand[at] = top_entry(ef, ee);
-  }
-  uint32_t hits = 0;
+  // the wavefront's vectors that reach the bound, from registers into LDS
+  const int w0 = (tid >> 6) * TOP_WAVE;
+  int n_vec = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if (i * 256 < rs.n) hits |= (vm[i] >= thr && i * 256 + tid < rs.n ? 1u : 0u) << i;
-  while (hits) {
-    const int s = (__ffs(hits) - 1) * 256 + tid;
-    hits &= hits - 1;
-    const RowVec<D> w = rs.load(p, s);
-    for (int j = 0; j < D::EPV; ++j) {
-      const float f = w.get(j);
-      if (f >= thr) {
-        const int at = atomicAdd(&n_cand, 1);
-        if (at < TOP_CAND) cand[at] = top_entry(f, rs.elem(s) + j);
+  for (int i = 0; i < NV; ++i) {
+    const bool hit = vm[i] >= thr && i * 256 + tid < rs.n;
+    const uint64_t all = __ballot(hit);
+    if (all) {
+      const int at = n_vec + lanes_below(all);
+      if (hit && at < TOP_WAVE) {
+        vec_slot[w0 + at] = i * 256 + tid;
+        vec_data[w0 + at] = make_uint4(v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]);
       }
+      n_vec += __popcll(all);
     }
+    __builtin_amdgcn_sched_barrier(0);
   }
-
-  m = fmaxf(m, -FLT_MAX);
   float sum = exp_t(ef - m, c);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -173,12 +207,39 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
     __builtin_amdgcn_sched_barrier(0);
   }
   const double ws = wave_sum_d((double)sum);
-  if (lane == 0) red[tid >> 6] = ws;
+  // their elements, one to a lane
+  wave_lds_fence();
+  int n_own = 0;
+  {
+    const bool hit = ef >= thr && ee >= 0;
+    const uint64_t all = __ballot(hit);
+    if (hit) cand[w0 + lanes_below(all)] = top_entry(ef, ee);
+    n_own = __popcll(all);
+  }
+  const uint32_t* words = (const uint32_t*)(vec_data + w0);
+  for (int base = 0; base < min(n_vec, TOP_WAVE) * D::EPV; base += 64) {
+    const int q = base + lane;
+    bool hit = q < min(n_vec, TOP_WAVE) * D::EPV;
+    float f = 0.f;
+    if (hit) {
+      f = D::unpack(words[q / RowVec<D>::PER], q % RowVec<D>::PER);
+      hit = f >= thr;
+    }
+    const uint64_t all = __ballot(hit);
+    const int at = n_own + lanes_below(all);
+    if (hit && at < TOP_WAVE) cand[w0 + at] = top_entry(f, rs.elem(vec_slot[w0 + q / D::EPV]) + q % D::EPV);
+    n_own += __popcll(all);
+  }
+  if (lane == 0) {
+    red[tid >> 6] = ws;
+    cnt[tid >> 6] = max(n_own, n_vec);                          // (a vector that does not fit has an element that does not)
+  }
   __syncthreads();
   const double s = (red[0] + red[1]) + (red[2] + red[3]);
-  int n = n_cand;
+  int n[4] = {cnt[0], cnt[1], cnt[2], cnt[3]};
 
-  if (s != s || n > TOP_CAND) {                                 // (from memory again: a copy in registers would cost every row its place)
+  const bool exact = s != s || max(max(n[0], n[1]), max(n[2], n[3])) > TOP_WAVE;
+  if (exact) {                                 // (from memory again: a copy in registers would cost every row its place)
     constexpr int SHIFT = D::KEY_ZEROS;
     auto count = [&](uint64_t at_least) {                       // elements with key >> SHIFT at or above
       int q = ee >= 0 && (order_key(ef) >> SHIFT) >= at_least ? 1 : 0;
@@ -244,49 +305,75 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
       }
     }
     __syncthreads();
-    n = kk;
+    n[0] = kk;
+    n[1] = n[2] = n[3] = 0;
   }
 
   if (n_chunk == 1) {
-    rank_out<256>(cand, n, k, [&](int rank, uint64_t o) {
+    rank_out<256, 4, TOP_WAVE>(cand, n, k, [&](int rank, uint64_t o) {
       index[r * k + rank] = entry_id(o);
       values[r * k + rank] = D::put(key_value((uint32_t)(o >> 32)));
     });
-    if (tid == 0) lse[r] = (float)((double)m * inv_temp + log(s));
-  } else {
-    uint64_t* l = lists + (int64_t)blockIdx.x * k;
-    rank_out<256>(cand, n, k, [&](int rank, uint64_t o) { l[rank] = o; });
-    for (int i = kk + tid; i < k; i += 256) l[i] = 0;
-    if (tid == 0) parts[blockIdx.x] = {(double)m, s};
+    if (tid == 0) lse[r] = (float)((double)m * inv_temp + logf((float)s));
+  } else {                                                      // unordered, all of them where they fit
+    uint64_t* l = lists + (int64_t)blockIdx.x * len;
+    int all = (n[0] + n[1]) + (n[2] + n[3]);
+    if (all <= len) {
+      int before = 0;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        for (int i = tid; i < n[g]; i += 256) l[before + i] = cand[g * TOP_WAVE + i];
+        before += n[g];
+      }
+    } else {
+      rank_out<256, 4, TOP_WAVE>(cand, n, k, [&](int rank, uint64_t o) { l[rank] = o; });
+      all = kk;
+    }
+    for (int i = all + tid; i < len; i += 256) l[i] = 0;
+    if (tid == 0) parts[blockIdx.x] = {(double)m, s, exact || kk < k ? -INFINITY : thr};
   }
 }
 
-// The lists of a row's chunks joined: 16 entries a thread, bisection until between k and TOP_CAND of them are left, ranks by counting.
+// The lists of a row's chunks joined: 16 entries a thread, bisection until between k and 5 k / 4 + 32 of them are left, ranks by counting.
 template <class D, int NT>
-__global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __restrict__ lists, const MaxSumD* __restrict__ parts,
+__global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __restrict__ lists, const TopPart* __restrict__ parts,
                                                            typename D::store* __restrict__ values, int64_t* __restrict__ index,
-                                                           float* __restrict__ lse, int k, int n_chunk, double inv_temp) {
-  __shared__ uint64_t cand[TOP_CAND];
+                                                           float* __restrict__ lse, int k, int len, int n_chunk, double inv_temp) {
+  __shared__ uint64_t cand[TOP_MAX_K + TOP_MAX_K / 4 + 32];
   __shared__ int cnt[NT / 64];
   __shared__ int n_cand;
   const int64_t r = blockIdx.x;
-  const int n = n_chunk * k;
+  const int n = n_chunk * len;
   uint64_t o[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = i * NT + (int)threadIdx.x < n ? lists[r * n + i * NT + threadIdx.x] : 0;
   if (threadIdx.x == 0) n_cand = 0;
-  uint64_t b0 = 1;
-  if (n > TOP_CAND) {
-    uint64_t b1 = ~0ull;                                        // above every entry: ids are below 2^24
+  // at least k entries reach the largest of the chunks' bounds
+  float bound = -INFINITY, top = -INFINITY;
+  for (int i = threadIdx.x & 63; i < n_chunk; i += 64) {
+    bound = fmaxf(bound, parts[r * n_chunk + i].bound);
+    top = fmaxf(top, (float)parts[r * n_chunk + i].m);
+  }
+  bound = wave_max(bound);
+  top = wave_max(top);
+  uint64_t b0 = bound > -INFINITY ? (uint64_t)order_key(bound) << 32 : 1;
+  if (n > k + k / 4 + 32) {
+    uint64_t b1 = bound > -INFINITY ? (uint64_t)(order_key(top) + 1) << 32 : ~0ull;   // above all entries, or not below the largest
     while (b1 - b0 > 1) {
       const uint64_t mid = b0 + ((b1 - b0) >> 1);
       int q = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) q += o[i] >= mid ? 1 : 0;
-      q = block_count<NT>(q, cnt);
+      for (int i = 0; i < 16; ++i)
+        if (i * NT < n) q += __popcll(__ballot(o[i] >= mid));
+      __syncthreads();
+      if ((threadIdx.x & 63) == 0) cnt[threadIdx.x >> 6] = q;
+      __syncthreads();
+      q = 0;
+#pragma unroll
+      for (int i = 0; i < NT / 64; ++i) q += cnt[i];
       if (q >= k) {
         b0 = mid;
-        if (q <= TOP_CAND) break;
+        if (q <= k + k / 4 + 32) break;
       } else {
         b1 = mid;
       }
@@ -297,7 +384,8 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
   for (int i = 0; i < 16; ++i)
     if (o[i] >= b0) cand[atomicAdd(&n_cand, 1)] = o[i];
   __syncthreads();
-  rank_out<NT>(cand, n_cand, k, [&](int rank, uint64_t q) {
+  const int left[1] = {n_cand};
+  rank_out<NT, 1, 0>(cand, left, k, [&](int rank, uint64_t q) {
     index[r * k + rank] = entry_id(q);
     values[r * k + rank] = D::put(key_value((uint32_t)(q >> 32)));
   });
@@ -311,51 +399,64 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
   }
 }
 
-// A chunk holds at most 16 vectors a thread, and not less than 16 k elements (or its list would be most of it).
-static int top_chunks(int rows, int V, int k, int dtype) {
-  const int n = row_chunks(rows, V, 256 * 16 * (16 / row_size(dtype)), 16 * k > 2048 ? 16 * k : 2048);
-  return n * k <= TOP_MAX_LIST ? n : row_chunks(512, V, 256 * 16 * (16 / row_size(dtype)), 1);
+// A chunk holds at most 16 vectors a thread, and not less than 16 k elements (or its list would be most of it).  Its list has room
+// for the candidates that a bound met by 5/4 k + 8 groups lets through, and at least k entries.
+struct TopPlan {
+  int n, chunk, len;
+};
+static TopPlan top_plan(int rows, int V, int k, int dtype) {
+  const int most = 256 * 16 * (16 / row_size(dtype));
+  TopPlan t;
+  t.n = row_chunks(rows, V, most, 16 * k > 2048 ? 16 * k : 2048);
+  if (t.n * k > TOP_MAX_LIST) t.n = row_chunks(512, V, most, V);
+  t.chunk = (V + t.n - 1) / t.n;
+  t.len = 2 * k + 32 < TOP_MAX_LIST / t.n ? 2 * k + 32 : TOP_MAX_LIST / t.n;
+  return t;
 }
 
 extern "C" int64_t nast_top_logits_workspace_bytes(int rows, int V, int k, int dtype) {
-  if (rows < 1 || V < 1 || k < 1 || !row_dtype_ok(dtype)) return 0;
-  const int64_t n = top_chunks(rows, V, k, dtype);
-  return n > 1 ? rows * n * (k * (int64_t)sizeof(uint64_t) + (int64_t)sizeof(MaxSumD)) : 0;
+  if (rows < 1 || V < 1 || V > TOP_MAX_V || k < 1 || k > TOP_MAX_K || !row_dtype_ok(dtype)) return 0;
+  const TopPlan t = top_plan(rows, V, k, dtype);
+  return t.n > 1 ? (int64_t)rows * t.n * (t.len * (int64_t)sizeof(uint64_t) + (int64_t)sizeof(TopPart)) : 0;
 }
 
 template <class D, int NV>
-static void top_launch(const void* x, nast_rows xr, void* values, int64_t* index, float* lse, uint64_t* lists, MaxSumD* parts, int rows,
-                       int V, int k, int chunk, int n, double temp, hipStream_t s) {
-  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NV>), dim3(rows * n), dim3(256), 0, s, (const typename D::store*)x, xr,
-                     (typename D::store*)values, index, lse, lists, parts, V, k, chunk, n, 1.0 / temp, exp_scale(temp));
-  if (n > 1 && n * k <= 4096)
-    hipLaunchKernelGGL((nast_top_join_kernel<D, 256>), dim3(rows), dim3(256), 0, s, lists, parts, (typename D::store*)values, index, lse, k, n,
+static void top_launch(const void* x, nast_rows xr, void* values, int64_t* index, float* lse, uint64_t* lists, TopPart* parts, int rows,
+                       int V, int k, TopPlan t, double temp, hipStream_t s) {
+  using T = typename D::store;
+  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NV>), dim3(rows * t.n), dim3(256), 0, s, (const T*)x, xr, (T*)values, index, lse, lists, parts,
+                     V, k, t.len, t.chunk, t.n, 1.0 / temp, exp_scale(temp));
+  if (t.n == 1) return;
+  if (t.n * t.len <= 4096)
+    hipLaunchKernelGGL((nast_top_join_kernel<D, 256>), dim3(rows), dim3(256), 0, s, lists, parts, (T*)values, index, lse, k, t.len, t.n,
                        1.0 / temp);
-  else if (n > 1)
-    hipLaunchKernelGGL((nast_top_join_kernel<D, 1024>), dim3(rows), dim3(1024), 0, s, lists, parts, (typename D::store*)values, index, lse, k,
-                       n, 1.0 / temp);
+  else
+    hipLaunchKernelGGL((nast_top_join_kernel<D, 1024>), dim3(rows), dim3(1024), 0, s, lists, parts, (T*)values, index, lse, k, t.len, t.n,
+                       1.0 / temp);
 }
 
 extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* values, int64_t* index, float* lse, int rows, int V,
                                int k, double temp, void* workspace, void* stream) {
   NAST_REQUIRE(row_dtype_ok(dtype), "nast_top_logits: unknown dtype %d", dtype);
-  NAST_REQUIRE(rows >= 0 && V >= 1 && V <= (1 << 20), "nast_top_logits: bad sizes rows=%d V=%d", rows, V);
+  NAST_REQUIRE(rows >= 0 && V >= 1 && V <= TOP_MAX_V, "nast_top_logits: bad sizes rows=%d V=%d", rows, V);
   NAST_REQUIRE(k >= 1 && k <= TOP_MAX_K && k <= V, "nast_top_logits: k=%d must lie in [1, %d] and not exceed V=%d", k, TOP_MAX_K, V);
   NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_top_logits: temperature must be > 0 and finite");
   if (rows == 0) return NAST_OK;
-  const int n = top_chunks(rows, V, k, dtype), chunk = (V + n - 1) / n;
-  NAST_REQUIRE((int64_t)rows * n < (1 << 22), "nast_top_logits: too many rows (%d)", rows);
-  NAST_REQUIRE(x && values && index && lse && (n == 1 || workspace), "nast_top_logits: NULL pointer");
+  const TopPlan t = top_plan(rows, V, k, dtype);
+  NAST_REQUIRE((int64_t)rows * t.n < (1 << 22), "nast_top_logits: too many rows (%d)", rows);
+  NAST_REQUIRE(x && values && index && lse && (t.n == 1 || workspace), "nast_top_logits: NULL pointer");
   NAST_REQUIRE(row_aligned(x, dtype) && row_aligned(values, dtype), "nast_top_logits: misaligned pointer");
   hipStream_t s = (hipStream_t)stream;
   uint64_t* lists = (uint64_t*)workspace;
-  MaxSumD* parts = n > 1 ? (MaxSumD*)(lists + (int64_t)rows * n * k) : nullptr;
-  const int nv = (chunk / (16 / row_size(dtype)) + 255) / 256;      // vectors a thread
+  TopPart* parts = t.n > 1 ? (TopPart*)(lists + (int64_t)rows * t.n * t.len) : nullptr;
+  const int nv = (t.chunk / (16 / row_size(dtype)) + 255) / 256;      // vectors a thread
   nast_prof_before(2, s);
-#define NAST_TOP(NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, chunk, n, temp, s)))
+#define NAST_TOP(NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, t, temp, s)))
   if (nv <= 2) NAST_TOP(2);
   else if (nv <= 4) NAST_TOP(4);
+  else if (nv <= 6) NAST_TOP(6);
   else if (nv <= 8) NAST_TOP(8);
+  else if (nv <= 10) NAST_TOP(10);
   else if (nv <= 12) NAST_TOP(12);
   else NAST_TOP(16);
 #undef NAST_TOP
@@ -416,8 +517,7 @@ __device__ void distill_finish(int64_t r, MaxSumD rest, const typename D::store*
       ids[j] = id[i];
     }
   }
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  wave_lds_fence();
   tm = wave_max(tm);
   const double M = fmax(rest.m, (double)wave_max(zm));
   double ts = 0, zs = 0, any = 0;
@@ -484,7 +584,8 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
   const int lo = (int)(block % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
   const RowSpan16<D> rs(p, lo, hi);
-  const int bit0 = rs.body - D::EPV;
+  const int bit0 = rs.body - D::EPV, e = rs.edge(threadIdx.x);
+  const typename D::store edge = p[e >= 0 ? e : lo];
   for (int w = threadIdx.x; w < (hi - bit0 + 31) / 32; w += 256) bits[w] = 0;
   __syncthreads();
   for (int j = threadIdx.x; j < K; j += 256) {
@@ -494,31 +595,34 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
   }
   __syncthreads();
   MaxSum a{-FLT_MAX, 0.f};
-  for (int base = threadIdx.x; base < rs.n; base += 256 * U) {
-    RowVec<D> v[U];
+  auto leave_out = [&](RowVec<D>& v, int slot) {
+    const int at = (slot + 1) * D::EPV;
+    const uint32_t named = bits[at >> 5] >> (at & 31) & ((1u << D::EPV) - 1);
+    if (named) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      v[u] = vec_of<D>(-INFINITY);
-      if (base + 256 * u < rs.n) v[u] = rs.load(p, base + 256 * u);
-    }
+      for (int i = 0; i < 4; ++i) {
+        float f[2];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = (base + 256 * u + 1) * D::EPV;
-      const uint32_t named = base + 256 * u < rs.n ? bits[at >> 5] >> (at & 31) & ((1u << D::EPV) - 1) : 0;
-      if (named) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float f[2];
-#pragma unroll
-          for (int j = 0; j < RowVec<D>::PER; ++j) f[j] = named >> (i * RowVec<D>::PER + j) & 1 ? -INFINITY : D::unpack(v[u].w[i], j);
-          v[u].w[i] = D::pack(f);
-        }
+        for (int j = 0; j < RowVec<D>::PER; ++j) f[j] = named >> (i * RowVec<D>::PER + j) & 1 ? -INFINITY : D::unpack(v.w[i], j);
+        v.w[i] = D::pack(f);
       }
     }
+  };
+  int base = threadIdx.x;
+  for (; base + 256 * (U - 1) < rs.n; base += 256 * U) {
+    RowVec<D> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + 256 * u);
+#pragma unroll
+    for (int u = 0; u < U; ++u) leave_out(v[u], base + 256 * u);
     fold<D, U>(a, v, c);
   }
-  const int e = rs.edge(threadIdx.x);
-  if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(p[e]), c);
+  for (; base < rs.n; base += 256) {
+    RowVec<D> v[1] = {rs.load(p, base)};
+    leave_out(v[0], base);
+    fold<D, 1>(a, v, c);
+  }
+  if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(edge), c);
   const MaxSumD rest = block_max_sum<256>(a, c, red);
   if (SPLIT) {
     if (threadIdx.x == 0) parts[block] = rest;
@@ -581,23 +685,28 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
   // a factor of 0 (a row without a list, a row of no weight) writes zeros whatever the logits hold
   const float F = gr == 0 ? 0.f : (float)(gr * st.coef), m = (float)st.m_rest;
   const RowSpan16<D> rs(o, lo, hi);
-  for (int base = threadIdx.x; base < rs.n; base += 256 * U) {
+  const int e = rs.edge(threadIdx.x);
+  const typename D::store edge = p[e >= 0 ? e : lo];
+  auto put = [&](RowVec<D>& v, int slot) {
+    float f[D::EPV];
+#pragma unroll
+    for (int i = 0; i < D::EPV; ++i) f[i] = F == 0.f ? 0.f : exp_t(v.get(i) - m, c) * F;
+    v.put(f);
+    vec_store<D>(o + rs.elem(slot), v);
+  };
+  int base = threadIdx.x;
+  for (; base + 256 * (U - 1) < rs.n; base += 256 * U) {
     RowVec<D> v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (base + 256 * u < rs.n) v[u] = vec_load_any<D>(p + rs.elem(base + 256 * u));
+    for (int u = 0; u < U; ++u) v[u] = vec_load_any<D>(p + rs.elem(base + 256 * u));
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (base + 256 * u >= rs.n) break;
-      float f[D::EPV];
-#pragma unroll
-      for (int i = 0; i < D::EPV; ++i) f[i] = F == 0.f ? 0.f : exp_t(v[u].get(i) - m, c) * F;
-      v[u].put(f);
-      vec_store<D>(o + rs.elem(base + 256 * u), v[u]);
-    }
+    for (int u = 0; u < U; ++u) put(v[u], base + 256 * u);
   }
-  const int e = rs.edge(threadIdx.x);
-  if (e >= 0) o[e] = D::put(F == 0.f ? 0.f : exp_t(D::get(p[e]) - m, c) * F);
+  for (; base < rs.n; base += 256) {
+    RowVec<D> v = vec_load_any<D>(p + rs.elem(base));
+    put(v, base);
+  }
+  if (e >= 0) o[e] = D::put(F == 0.f ? 0.f : exp_t(D::get(edge) - m, c) * F);
   __syncthreads();
   if (id == DISTILL_NO_ID) return;
   double pj = 0;
