@@ -469,8 +469,6 @@ extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* val
 // distillation
 // ---------------------------------------------------------------------------------------------
 #define DISTILL_MAX_K 256
-#define DISTILL_SLOTS (DISTILL_MAX_K / 64)
-#define DISTILL_CHUNK 32768       // elements one workgroup reads at most: 4 KB of membership bits
 #define DISTILL_NO_ID 0xffffffffu
 
 // teacher's list in its own type
@@ -488,87 +486,128 @@ struct DistillStats {
   double m_rest, coef, M, L, C, c;
 };
 
-// The end of a row's forward pass by ONE wavefront; slot j = lane + 64 * i.  m, s: maximum and exponential sum of the tokens that no
-// used slot names.  Everything here is in double: the loss is a small difference of terms near 1 (with one slot of p = 0.01 and
-// q = 0.0075 it is 3e-4, while p_r log p_r alone is rounded by 6e-8 in fp32), and it is a few slots per row.
-template <class D>
-__device__ void distill_finish(int64_t r, MaxSumD rest, const typename D::store* p, const void* t, int t_dtype,
-                               const int64_t* idx, int K, const float* lse_t, float* loss, DistillStats* stats, int V, double it,
-                               uint32_t* ids) {
-  const int lane = threadIdx.x & 63;
-  float tj[DISTILL_SLOTS], zj[DISTILL_SLOTS];
-  uint32_t id[DISTILL_SLOTS];
-  float tm = -FLT_MAX, zm = -FLT_MAX;
+// What the list alone contributes to a row: with d_j = log p_j - (z_j - zm) / T up to the normalisers not known yet,
+//   S0 = sum e_j, S1 = sum e_j d_j, S2 = sum of exp((z - zm) / T) over the tokens named (each once), e_j = exp((t_j - C) / T - c0).
+// In double throughout: the loss is a small difference of terms near 1 (with one slot of p = 0.01 and q = 0.0075 it is 3e-4, while
+// p_r log p_r alone is rounded by 6e-8 in fp32), and it is a few slots per row.
+struct SlotSums {
+  double S0, S1, S2, C, c0, zm;
+  bool any;
+};
+
+// By a workgroup of NT >= K threads, thread j = slot j; every thread gets the sums.  ids: LDS, holds the used slots' ids afterwards.
+// Without TAIL no S2.
+template <class D, int NT, bool TAIL>
+__device__ __forceinline__ SlotSums slot_sums(int64_t r, const typename D::store* p, const void* t, int t_dtype, const int64_t* idx, int K,
+                                              const float* lse_t, int V, double it, uint32_t* ids, double* red) {
+  constexpr int W = NT / 64;
+  const int j = threadIdx.x, w = threadIdx.x >> 6;
+  uint32_t id = DISTILL_NO_ID;
+  float tj = -INFINITY, zj = -INFINITY;
+  if (j < K) {
+    const int64_t v = idx[r * K + j];
+    tj = teacher_logit(t, t_dtype, r * K + j);
+    if (slot_used(v, tj, V)) {
+      id = (uint32_t)v;
+      zj = D::get(p[v]);
+    }
+    ids[j] = id;
+  }
+  const bool used = id != DISTILL_NO_ID;
+  float tm = wave_max(used ? tj : -FLT_MAX), zm = wave_max(used ? zj : -FLT_MAX);
+  tm = fmaxf(tm, -FLT_MAX);
+  zm = fmaxf(zm, -FLT_MAX);
+  if ((j & 63) == 0) {
+    red[2 * w] = tm;
+    red[2 * w + 1] = zm;
+  }
+  __syncthreads();
+  SlotSums q;
+  double top = red[0];
+  q.zm = red[1];
 #pragma unroll
-  for (int i = 0; i < DISTILL_SLOTS; ++i) {
-    const int j = lane + 64 * i;
-    id[i] = DISTILL_NO_ID;
-    tj[i] = zj[i] = -INFINITY;
-    if (j < K) {
-      const int64_t v = idx[r * K + j];
-      const float tv = teacher_logit(t, t_dtype, r * K + j);
-      if (slot_used(v, tv, V)) {
-        id[i] = (uint32_t)v;
-        tj[i] = tv;
-        zj[i] = D::get(p[v]);
-        tm = fmaxf(tm, tv);
-        zm = fmaxf(zm, zj[i]);
-      }
-      ids[j] = id[i];
+  for (int i = 1; i < W; ++i) {
+    top = fmax(top, red[2 * i]);
+    q.zm = fmax(q.zm, red[2 * i + 1]);
+  }
+  q.C = TAIL ? 0.0 : top;
+  q.c0 = TAIL ? (double)lse_t[r] : 0.0;
+  double e = 0, ed = 0, ez = 0;
+  if (used) {
+    const double a = ((double)tj - q.C) * it - q.c0, b = ((double)zj - q.zm) * it;
+    e = exp(a);
+    if (e != 0) ed = e * (a - b);
+    if (TAIL) {
+      bool first = true;                     // an id named twice is one token of the student's
+      for (int i = 0; i < j; ++i) first = first && ids[i] != id;
+      if (first) ez = exp(b);
     }
   }
-  wave_lds_fence();
-  tm = wave_max(tm);
-  const double M = fmax(rest.m, (double)wave_max(zm));
-  double ts = 0, zs = 0, any = 0;
+  double any = __ballot(used) ? 1 : 0;
+  if (any != 0) {
+    e = wave_sum_d(e);
+    ed = wave_sum_d(ed);
+    if (TAIL) ez = wave_sum_d(ez);
+  }
+  __syncthreads();
+  if ((j & 63) == 0) {
+    red[4 * w] = e;
+    red[4 * w + 1] = ed;
+    red[4 * w + 2] = ez;
+    red[4 * w + 3] = any;
+  }
+  __syncthreads();
+  q.S0 = q.S1 = q.S2 = 0;
+  q.any = false;
 #pragma unroll
-  for (int i = 0; i < DISTILL_SLOTS; ++i) {
-    if (id[i] == DISTILL_NO_ID) continue;
-    any = 1;
-    ts += exp(((double)tj[i] - tm) * it);
-    bool first = true;                       // an id named twice is one token of the student's
-    for (int j = 0; j < lane + 64 * i; ++j) first = first && ids[j] != id[i];
-    if (first) zs += exp(((double)zj[i] - M) * it);
+  for (int i = 0; i < W; ++i) {
+    q.S0 += red[4 * i];
+    q.S1 += red[4 * i + 1];
+    q.S2 += red[4 * i + 2];
+    q.any = q.any || red[4 * i + 3] != 0;
   }
-  ts = wave_sum_d(ts);
-  zs = wave_sum_d(zs);
-  any = wave_max_d(any);
-  const double sr = rest.s * exp((rest.m - M) * it);
-  const double L = log(zs + sr), C = lse_t ? 0.0 : (double)tm, c = lse_t ? (double)lse_t[r] : log(ts);
-  double sum_p = 0, l = 0;
-#pragma unroll
-  for (int i = 0; i < DISTILL_SLOTS; ++i) {
-    if (id[i] == DISTILL_NO_ID) continue;
-    const double logp = ((double)tj[i] - C) * it - c, pj = exp(logp);
-    sum_p += pj;
-    if (pj != 0) l += pj * (logp - (((double)zj[i] - M) * it - L));
-  }
-  sum_p = wave_sum_d(sum_p);
-  l = wave_sum_d(l);
-  const double log_qr = (rest.m - M) * it + log(rest.s) - L, qr = exp(log_qr);
-  double pr = lse_t ? fmax(1.0 - sum_p, 0.0) : 0.0;
-  if (rest.s == 0) pr = 0;                   // no token of the student's is left for the bucket
-  if (pr > 0) l += pr * (log(pr) - log_qr);
-  if (lane == 0) {
-    DistillStats o;
-    o.m_rest = rest.m;
-    o.M = M;
-    o.L = L;
-    o.C = C;
-    o.c = c;
-    // q_v - p_r q_v / q_r = exp((z_v - m_r) / T) / s_r * (q_r - p_r): no quotient of small numbers; 0 for a row without a list and
-    // for one without a rest, NaN for a row of nothing but -inf
-    o.coef = any == 0 ? 0.0 : rest.s == 0 ? (L > -INFINITY ? 0.0 : NAN) : (qr - pr) / rest.s;
-    stats[r] = o;
-    loss[r] = any == 0 ? 0.f : (float)l;
-  }
+  __syncthreads();
+  return q;
 }
 
-// One workgroup per chunk of a row: (max, exponential sum) of the tokens that no used slot names.  The named ones are marked in LDS,
-// one bit per element, and left out of both: their terms are added in double at the end, and q_r is a sum and no difference.
+// The end of a row's forward pass by one thread.  rest: maximum and exponential sum, with TAIL of the tokens that no used slot names,
+// without of all.
+template <bool TAIL>
+__device__ __forceinline__ void distill_finish(int64_t r, const MaxSumD& rest, const SlotSums& q, float* loss, DistillStats* stats, double it) {
+  DistillStats o;
+  double l;
+  o.m_rest = rest.m;
+  o.C = q.C;
+  if (TAIL) {
+    o.M = fmax(rest.m, q.zm);
+    const double below = (rest.m - o.M) * it;
+    o.L = log(q.S2 * exp((q.zm - o.M) * it) + rest.s * exp(below));
+    o.c = q.c0;
+    l = q.S1 + q.S0 * ((o.M - q.zm) * it + o.L);
+    const double log_qr = below + log(rest.s) - o.L;
+    const double pr = rest.s == 0 ? 0.0 : fmax(1.0 - q.S0, 0.0);   // (no bucket where the student has no token left for it)
+    if (pr > 0) l += pr * (log(pr) - log_qr);
+    // q_v - p_r q_v / q_r = exp((z_v - m_r) / T) / s_r * (q_r - p_r): no quotient of small numbers; 0 for a row without a rest, NaN
+    // for a row of nothing but -inf
+    o.coef = rest.s == 0 ? (o.L > -INFINITY ? 0.0 : NAN) : (exp(log_qr) - pr) / rest.s;
+  } else {
+    o.M = rest.m;
+    o.L = log(rest.s);
+    o.c = log(q.S0);
+    l = q.S1 / q.S0 - o.c + (o.M - q.zm) * it + o.L;
+    o.coef = rest.s == 0 ? NAN : 1.0 / rest.s;
+  }
+  if (!q.any) o.coef = l = 0;
+  stats[r] = o;
+  loss[r] = (float)l;
+}
+
+// One workgroup per chunk of a row: (max, exponential sum) of its tokens; with TAIL of those that no used slot names.  The named ones are
+// marked in LDS, one bit per element and one per vector, and left out: their terms are added in double at the end, so that q_r is a sum
+// and no difference.
 // Rows are taken from the last to the first: the backward pass, from the first to the last, then begins with what this pass has
 // left in the last-level cache (256 MB), and this pass with what the product that made the logits has left there.
-template <class D, bool SPLIT>
+template <class D, bool SPLIT, bool TAIL>
 __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                                    const void* __restrict__ t, int t_dtype,
                                                                    const int64_t* __restrict__ idx, int K,
@@ -576,29 +615,44 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
                                                                    DistillStats* __restrict__ stats, MaxSumD* __restrict__ parts, int V,
                                                                    int chunk, int n_chunk, double it, float c) {
   constexpr int U = 4;
-  __shared__ uint32_t bits[DISTILL_CHUNK / 32 + 2];            // bit EPV + i: element body + i
-  __shared__ double red[8];
+  extern __shared__ uint32_t bits[];                           // bit EPV + i: element body + i
+  __shared__ double red[16];
   __shared__ uint32_t ids[DISTILL_MAX_K];
   const unsigned block = gridDim.x - 1 - blockIdx.x;
   const int64_t r = block / n_chunk;
   const int lo = (int)(block % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
-  const RowSpan16<D> rs(p, lo, hi);
-  const int bit0 = rs.body - D::EPV, e = rs.edge(threadIdx.x);
-  const typename D::store edge = p[e >= 0 ? e : lo];
-  for (int w = threadIdx.x; w < (hi - bit0 + 31) / 32; w += 256) bits[w] = 0;
-  __syncthreads();
-  for (int j = threadIdx.x; j < K; j += 256) {
-    const int64_t id = idx[r * K + j];
-    if (id >= lo && id < hi && slot_used(id, teacher_logit(t, t_dtype, r * K + j), V))
-      atomicOr(&bits[(id - bit0) >> 5], 1u << ((id - bit0) & 31));
-  }
-  __syncthreads();
   MaxSum a{-FLT_MAX, 0.f};
-  auto leave_out = [&](RowVec<D>& v, int slot) {
-    const int at = (slot + 1) * D::EPV;
-    const uint32_t named = bits[at >> 5] >> (at & 31) & ((1u << D::EPV) - 1);
-    if (named) {
+  SlotSums q;
+  if (!SPLIT) q = slot_sums<D, 256, TAIL>(r, p, t, t_dtype, idx, K, lse_t, V, it, ids, red);
+  if (!TAIL) {
+    a = span_max_sum<D, 256>(p, lo, hi, c);
+  } else {
+    const RowSpan16<D> rs(p, lo, hi);
+    const int bit0 = rs.body - D::EPV, e = rs.edge(threadIdx.x), words = (hi - bit0 + 31) / 32;
+    const typename D::store edge = p[e >= 0 ? e : lo];
+    uint32_t* flags = bits + words;                            // byte (s / 1024) * 256 + s % 256, bit s / 256 % 4: vector s
+    const int flag_words = (rs.n + 1023) / 1024 * 64;
+    for (int w = threadIdx.x; w < words + flag_words; w += 256) bits[w] = 0;
+    uint32_t id = DISTILL_NO_ID;
+    if ((int)threadIdx.x < K) {
+      if (SPLIT) {
+        const int64_t v = idx[r * K + threadIdx.x];
+        if (v >= lo && v < hi && slot_used(v, teacher_logit(t, t_dtype, r * K + threadIdx.x), V)) id = (uint32_t)v;
+      } else {
+        id = ids[threadIdx.x];
+      }
+    }
+    __syncthreads();
+    if (id != DISTILL_NO_ID) {
+      const int bit = (int)id - bit0, s = ((int)id - rs.body) / D::EPV;
+      atomicOr(&bits[bit >> 5], 1u << (bit & 31));
+      if ((int)id >= rs.body && s < rs.n) atomicOr(&flags[(s >> 10) * 64 + ((s & 255) >> 2)], 1u << ((s & 3) * 8 + ((s >> 8) & 3)));
+    }
+    __syncthreads();
+    auto leave_out = [&](RowVec<D>& v, int slot) {
+      const int at = (slot + 1) * D::EPV;
+      const uint32_t named = bits[at >> 5] >> (at & 31);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float f[2];
@@ -606,51 +660,55 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
         for (int j = 0; j < RowVec<D>::PER; ++j) f[j] = named >> (i * RowVec<D>::PER + j) & 1 ? -INFINITY : D::unpack(v.w[i], j);
         v.w[i] = D::pack(f);
       }
+    };
+    const uint8_t* flag = (const uint8_t*)flags + threadIdx.x;
+    int base = threadIdx.x;
+    for (; base + 256 * (U - 1) < rs.n; base += 256 * U, flag += 256) {
+      RowVec<D> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + 256 * u);
+      const uint32_t f = *flag;
+      if (f) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (f >> u & 1) leave_out(v[u], base + 256 * u);
+      }
+      fold<D, U>(a, v, c);
     }
-  };
-  int base = threadIdx.x;
-  for (; base + 256 * (U - 1) < rs.n; base += 256 * U) {
-    RowVec<D> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + 256 * u);
-#pragma unroll
-    for (int u = 0; u < U; ++u) leave_out(v[u], base + 256 * u);
-    fold<D, U>(a, v, c);
+    for (; base < rs.n; base += 256) {
+      RowVec<D> v[1] = {rs.load(p, base)};
+      leave_out(v[0], base);
+      fold<D, 1>(a, v, c);
+    }
+    if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(edge), c);
   }
-  for (; base < rs.n; base += 256) {
-    RowVec<D> v[1] = {rs.load(p, base)};
-    leave_out(v[0], base);
-    fold<D, 1>(a, v, c);
-  }
-  if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(edge), c);
   const MaxSumD rest = block_max_sum<256>(a, c, red);
-  if (SPLIT) {
-    if (threadIdx.x == 0) parts[block] = rest;
-  } else if (threadIdx.x < 64) {
-    distill_finish<D>(r, rest, p, t, t_dtype, idx, K, lse_t, loss, stats, V, it, ids);
-  }
+  if (threadIdx.x != 0) return;
+  if (SPLIT) parts[block] = rest;
+  else distill_finish<TAIL>(r, rest, q, loss, stats, it);
 }
 
-// one wavefront per row joins the chunks
-template <class D>
-__global__ __launch_bounds__(64) void nast_top_distill_join_kernel(const typename D::store* __restrict__ x, nast_rows xr,
+// one workgroup of NT >= K threads per row joins the chunks
+template <class D, int NT, bool TAIL>
+__global__ __launch_bounds__(NT) void nast_top_distill_join_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                                    const void* __restrict__ t, int t_dtype,
                                                                    const int64_t* __restrict__ idx, int K,
                                                                    const float* __restrict__ lse_t, float* __restrict__ loss,
                                                                    DistillStats* __restrict__ stats, const MaxSumD* __restrict__ parts,
                                                                    int V, int n_chunk, double it) {
-  __shared__ uint32_t ids[DISTILL_MAX_K];
+  __shared__ double red[NT / 16];
+  __shared__ uint32_t ids[NT];
   const int64_t r = blockIdx.x;
   MaxSumD rest{-FLT_MAX, 0};
-  double m = -FLT_MAX, s = 0;
-  for (int i = threadIdx.x; i < n_chunk; i += 64) m = fmax(m, parts[r * n_chunk + i].m);
-  rest.m = wave_max_d(m);
-  for (int i = threadIdx.x; i < n_chunk; i += 64) {
-    const MaxSumD q = parts[r * n_chunk + i];
-    s += q.s * exp((q.m - rest.m) * it);
+  for (int i = threadIdx.x & 63; i < n_chunk; i += 64) rest.m = fmax(rest.m, parts[r * n_chunk + i].m);
+  rest.m = wave_max_d(rest.m);
+  for (int i = threadIdx.x & 63; i < n_chunk; i += 64) {
+    const MaxSumD o = parts[r * n_chunk + i];
+    rest.s += o.s * exp((o.m - rest.m) * it);
   }
-  rest.s = wave_sum_d(s);
-  distill_finish<D>(r, rest, x + row_offset(r, xr), t, t_dtype, idx, K, lse_t, loss, stats, V, it, ids);
+  rest.s = wave_sum_d(rest.s);
+  const SlotSums q = slot_sums<D, NT, TAIL>(r, x + row_offset(r, xr), t, t_dtype, idx, K, lse_t, V, it, ids, red);
+  if (threadIdx.x == 0) distill_finish<TAIL>(r, rest, q, loss, stats, it);
 }
 
 // One workgroup per chunk of a row: the rest's gradient everywhere, then, behind a barrier, the value of each named token over it.
@@ -726,11 +784,44 @@ static int distill_check(const char* name, int dtype, int t_dtype, int K, int ro
   NAST_REQUIRE(temp > 0 && temp < 1e30, "%s: temperature must be > 0 and finite", name);
   return NAST_OK;
 }
-static int distill_chunk(int rows, int V) { return V < DISTILL_CHUNK - 8 ? V : DISTILL_CHUNK - 8; }
+// One workgroup reads a whole row where there are rows enough to fill the card (512: two workgroups a compute unit); a chunk has 16 to
+// 256 Ki elements, 32 KB of membership bits at most.
+struct DistillPlan {
+  int n, chunk;
+};
+static DistillPlan distill_plan(int rows, int V) {
+  DistillPlan d;
+  d.n = row_chunks(rows, V, 1 << 18, 1 << 14);
+  d.chunk = (V + d.n - 1) / d.n;
+  return d;
+}
 
 extern "C" int64_t nast_top_distill_workspace_bytes(int rows, int V, int dtype) {
-  const int chunk = distill_chunk(rows, V), n = (V + chunk - 1) / chunk;
-  return n > 1 ? (int64_t)rows * n * (int64_t)sizeof(MaxSumD) : 0;
+  if (rows < 1 || V < 1) return 0;
+  const DistillPlan d = distill_plan(rows, V);
+  return d.n > 1 ? (int64_t)rows * d.n * (int64_t)sizeof(MaxSumD) : 0;
+}
+
+template <class D, bool TAIL>
+static void distill_fwd(const void* x, nast_rows xr, const void* t, int t_dtype, const int64_t* idx, int K, const float* lse_t,
+                        float* loss, DistillStats* st, MaxSumD* parts, int rows, int V, DistillPlan d, double temp, hipStream_t s) {
+  const typename D::store* xp = (const typename D::store*)x;
+  const double it = 1.0 / temp;
+  // bits of a chunk's elements, and of its vectors in fours of 256
+  const unsigned lds = TAIL ? 4u * ((d.chunk + 16 + 31) / 32 + (d.chunk / D::EPV + 1023) / 1024 * 64) : 0;
+  if (d.n == 1) {
+    hipLaunchKernelGGL((nast_top_distill_fwd_kernel<D, false, TAIL>), dim3(rows), dim3(256), lds, s, xp, xr, t, t_dtype, idx, K, lse_t, loss,
+                       st, parts, V, d.chunk, d.n, it, exp_scale(temp));
+    return;
+  }
+  hipLaunchKernelGGL((nast_top_distill_fwd_kernel<D, true, TAIL>), dim3(rows * d.n), dim3(256), lds, s, xp, xr, t, t_dtype, idx, K, lse_t,
+                     loss, st, parts, V, d.chunk, d.n, it, exp_scale(temp));
+  if (K <= 64)
+    hipLaunchKernelGGL((nast_top_distill_join_kernel<D, 64, TAIL>), dim3(rows), dim3(64), 0, s, xp, xr, t, t_dtype, idx, K, lse_t, loss, st,
+                       parts, V, d.n, it);
+  else
+    hipLaunchKernelGGL((nast_top_distill_join_kernel<D, 256, TAIL>), dim3(rows), dim3(256), 0, s, xp, xr, t, t_dtype, idx, K, lse_t, loss, st,
+                       parts, V, d.n, it);
 }
 
 extern "C" int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, const void* t, int t_dtype, const int64_t* idx, int K,
@@ -740,25 +831,16 @@ extern "C" int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, cons
   if (rows == 0) return NAST_OK;
   NAST_REQUIRE(x && t && idx && loss && stats, "nast_top_distill_fwd: NULL pointer");
   NAST_REQUIRE(row_aligned(x, dtype) && row_aligned(t, t_dtype), "nast_top_distill_fwd: misaligned pointer");
-  const int chunk = distill_chunk(rows, V), n = (V + chunk - 1) / chunk;
-  NAST_REQUIRE(n == 1 || workspace, "nast_top_distill_fwd: NULL workspace");
-  NAST_REQUIRE((int64_t)rows * n < (1 << 24), "nast_top_distill_fwd: too many rows (%d)", rows);
+  const DistillPlan d = distill_plan(rows, V);
+  NAST_REQUIRE((int64_t)rows * d.n < (1 << 24), "nast_top_distill_fwd: too many rows (%d)", rows);
+  NAST_REQUIRE(d.n == 1 || workspace, "nast_top_distill_fwd: NULL workspace");
   hipStream_t s = (hipStream_t)stream;
   DistillStats* st = (DistillStats*)stats;
   MaxSumD* parts = (MaxSumD*)workspace;
-  const float c = exp_scale(temp);
   nast_prof_before(2, s);
   NAST_ROW_DTYPE(dtype, {
-    const typename D::store* xp = (const typename D::store*)x;
-    if (n == 1) {
-      hipLaunchKernelGGL((nast_top_distill_fwd_kernel<D, false>), dim3(rows), dim3(256), 0, s, xp, xr, t, t_dtype, idx, K, lse_t, loss, st,
-                         parts, V, chunk, n, 1.0 / temp, c);
-    } else {
-      hipLaunchKernelGGL((nast_top_distill_fwd_kernel<D, true>), dim3(rows * n), dim3(256), 0, s, xp, xr, t, t_dtype, idx, K, lse_t, loss,
-                         st, parts, V, chunk, n, 1.0 / temp, c);
-      hipLaunchKernelGGL((nast_top_distill_join_kernel<D>), dim3(rows), dim3(64), 0, s, xp, xr, t, t_dtype, idx, K, lse_t, loss, st, parts,
-                         V, n, 1.0 / temp);
-    }
+    if (lse_t) distill_fwd<D, true>(x, xr, t, t_dtype, idx, K, lse_t, loss, st, parts, rows, V, d, temp, s);
+    else distill_fwd<D, false>(x, xr, t, t_dtype, idx, K, lse_t, loss, st, parts, rows, V, d, temp, s);
   });
   nast_prof_after(2, s, (double)row_size(dtype) * rows * (double)V);
   NAST_CHECK_LAUNCH("nast_top_distill_fwd");

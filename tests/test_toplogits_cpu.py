@@ -85,7 +85,7 @@ def test_c_entries_refuse():
     refused(*fwd(loss=None), match="NULL")
     refused(*fwd(x=P + 1, dtype=1), match="misaligned")
     refused(*fwd(rows=1, V=200000, ws=None), match="workspace")
-    refused(*fwd(rows=big - 1, V=200000), match="too many rows")
+    refused(*fwd(rows=big - 1, V=600000), match="too many rows")
     bwd = lambda g=P, x=P, gx=2 * P, rows=2, V=8: ("nast_top_distill_bwd", g, x, 0, R, P, 0, P, 3, P, gx, R, rows, V, 1.0, None)
     refused(*bwd(gx=P), match="in-place")
     refused(*bwd(g=None), match="NULL")
