@@ -129,25 +129,39 @@ __device__ __forceinline__ void fold_one(MaxSum& a, float f, float c) {
   a.s += exp_t(f - a.m, c);
 }
 
+// The slots of a span in batches of U vectors a thread: full(v, first slot) for a batch that every thread has whole, part(v, slot) for
+// each vector of the last one.  No branch around a load: the compiler would wait for each before the next.
+template <class D, int NT, int U, class L, class F, class P>
+__device__ __forceinline__ void for_slots(const RowSpan16<D>& rs, L&& load, F&& full, P&& part) {
+  const int tid = threadIdx.x;
+  int b = 0;
+  for (; b + NT * U <= rs.n; b += NT * U) {
+    RowVec<D> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load(b + NT * u + tid);
+    full(v, b + tid);
+  }
+  if (b >= rs.n) return;
+  RowVec<D> v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = load(min(b + NT * u + tid, rs.n - 1));
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (b + NT * u + tid < rs.n) part(v[u], b + NT * u + tid);
+}
+
 // a thread's share of elements [lo, hi) of a row
-template <class D, int NT>
+template <class D, int NT, int U = 4>
 __device__ __forceinline__ MaxSum span_max_sum(const typename D::store* p, int lo, int hi, float c) {
-  constexpr int U = 4;
   const RowSpan16<D> rs(p, lo, hi);
   const int e = rs.edge(threadIdx.x);
   const typename D::store edge = p[e >= 0 ? e : lo];
   MaxSum a{-FLT_MAX, 0.f};
-  int base = threadIdx.x;
-  for (; base + NT * (U - 1) < rs.n; base += NT * U) {     // (no branch around a load: the compiler would wait for each before the next)
-    RowVec<D> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + NT * u);
-    fold<D, U>(a, v, c);
-  }
-  for (; base < rs.n; base += NT) {
-    const RowVec<D> v[1] = {rs.load(p, base)};
-    fold<D, 1>(a, v, c);
-  }
+  for_slots<D, NT, U>(rs, [&](int s) { return rs.load(p, s); }, [&](const RowVec<D>(&v)[U], int) { fold<D, U>(a, v, c); },
+                      [&](const RowVec<D>& v, int) {
+                        const RowVec<D> one[1] = {v};
+                        fold<D, 1>(a, one, c);
+                      });
   if (e >= 0) fold_one(a, D::get(edge), c);
   return a;
 }

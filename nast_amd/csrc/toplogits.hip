@@ -661,25 +661,22 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
         v.w[i] = D::pack(f);
       }
     };
-    const uint8_t* flag = (const uint8_t*)flags + threadIdx.x;
-    int base = threadIdx.x;
-    for (; base + 256 * (U - 1) < rs.n; base += 256 * U, flag += 256) {
-      RowVec<D> v[U];
+    const uint8_t* flag = (const uint8_t*)flags;
+    for_slots<D, 256, U>(rs, [&](int s) { return rs.load(p, s); },
+                         [&](RowVec<D>(&v)[U], int s) {
+                           const uint32_t f = flag[(s >> 10) * 256 + threadIdx.x];
+                           if (f) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = rs.load(p, base + 256 * u);
-      const uint32_t f = *flag;
-      if (f) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (f >> u & 1) leave_out(v[u], base + 256 * u);
-      }
-      fold<D, U>(a, v, c);
-    }
-    for (; base < rs.n; base += 256) {
-      RowVec<D> v[1] = {rs.load(p, base)};
-      leave_out(v[0], base);
-      fold<D, 1>(a, v, c);
-    }
+                             for (int u = 0; u < U; ++u)
+                               if (f >> u & 1) leave_out(v[u], s + 256 * u);
+                           }
+                           fold<D, U>(a, v, c);
+                         },
+                         [&](RowVec<D>& v, int s) {
+                           leave_out(v, s);
+                           const RowVec<D> one[1] = {v};
+                           fold<D, 1>(a, one, c);
+                         });
     if (e >= 0 && !(bits[(e - bit0) >> 5] >> ((e - bit0) & 31) & 1)) fold_one(a, D::get(edge), c);
   }
   const MaxSumD rest = block_max_sum<256>(a, c, red);
@@ -752,18 +749,12 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
     v.put(f);
     vec_store<D>(o + rs.elem(slot), v);
   };
-  int base = threadIdx.x;
-  for (; base + 256 * (U - 1) < rs.n; base += 256 * U) {
-    RowVec<D> v[U];
+  for_slots<D, 256, U>(rs, [&](int s) { return vec_load_any<D>(p + rs.elem(s)); },
+                       [&](RowVec<D>(&v)[U], int s) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = vec_load_any<D>(p + rs.elem(base + 256 * u));
-#pragma unroll
-    for (int u = 0; u < U; ++u) put(v[u], base + 256 * u);
-  }
-  for (; base < rs.n; base += 256) {
-    RowVec<D> v = vec_load_any<D>(p + rs.elem(base));
-    put(v, base);
-  }
+                         for (int u = 0; u < U; ++u) put(v[u], s + 256 * u);
+                       },
+                       put);
   if (e >= 0) o[e] = D::put(F == 0.f ? 0.f : exp_t(D::get(edge) - m, c) * F);
   __syncthreads();
   if (id == DISTILL_NO_ID) return;
@@ -784,21 +775,21 @@ static int distill_check(const char* name, int dtype, int t_dtype, int K, int ro
   NAST_REQUIRE(temp > 0 && temp < 1e30, "%s: temperature must be > 0 and finite", name);
   return NAST_OK;
 }
-// One workgroup reads a whole row where there are rows enough to fill the card (512: two workgroups a compute unit); a chunk has 16 to
-// 256 Ki elements, 32 KB of membership bits at most.
+// One workgroup reads a whole row where there are rows enough to fill the card (512: two workgroups a compute unit); a chunk has at
+// least 16 Ki elements and at most 2^15 vectors: a thread's fp32 sum has 128 of them, the membership bits take 40 KB.
 struct DistillPlan {
   int n, chunk;
 };
-static DistillPlan distill_plan(int rows, int V) {
+static DistillPlan distill_plan(int rows, int V, int dtype) {
   DistillPlan d;
-  d.n = row_chunks(rows, V, 1 << 18, 1 << 14);
+  d.n = row_chunks(rows, V, (16 / row_size(dtype)) << 15, 1 << 14);
   d.chunk = (V + d.n - 1) / d.n;
   return d;
 }
 
 extern "C" int64_t nast_top_distill_workspace_bytes(int rows, int V, int dtype) {
-  if (rows < 1 || V < 1) return 0;
-  const DistillPlan d = distill_plan(rows, V);
+  if (rows < 1 || V < 1 || !row_dtype_ok(dtype)) return 0;
+  const DistillPlan d = distill_plan(rows, V, dtype);
   return d.n > 1 ? (int64_t)rows * d.n * (int64_t)sizeof(MaxSumD) : 0;
 }
 
@@ -831,7 +822,7 @@ extern "C" int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, cons
   if (rows == 0) return NAST_OK;
   NAST_REQUIRE(x && t && idx && loss && stats, "nast_top_distill_fwd: NULL pointer");
   NAST_REQUIRE(row_aligned(x, dtype) && row_aligned(t, t_dtype), "nast_top_distill_fwd: misaligned pointer");
-  const DistillPlan d = distill_plan(rows, V);
+  const DistillPlan d = distill_plan(rows, V, dtype);
   NAST_REQUIRE((int64_t)rows * d.n < (1 << 24), "nast_top_distill_fwd: too many rows (%d)", rows);
   NAST_REQUIRE(d.n == 1 || workspace, "nast_top_distill_fwd: NULL workspace");
   hipStream_t s = (hipStream_t)stream;

@@ -9,29 +9,29 @@
 // comparison is closer than they are, it is made again in double over the whole row.
 #include "rowvec.h"
 
-#define VERIFY_CHUNK 32768
+#define VERIFY_MAX_V (1 << 20)
 #define VERIFY_MAX_DRAFTS 1024
-#define VERIFY_REL 1e-5           // fp32 exponentials, sums and products here are within this, relative (see exp_t: ~1e-6)
-
-struct VerifyRows {               // rows [.., V] of a [B, n, V] tensor
-  int64_t bs, rs;
-};
+// What the fp32 probabilities here are off by, relative: sums of exponentials 1.6e-5 (at most 256 vectors of 4 a thread, one rounding
+// each), exponents of magnitude up to 126 three roundings each, 1.6e-5, and the instructions' own.
+#define VERIFY_REL 4e-5f
 
 struct VerifyArgs {
   const void *target, *draft;     // draft NULL: no probabilities
-  VerifyRows tr, qr;
+  int64_t t_bs, t_rs, q_bs, q_rs; // strides of batch and row
   const int64_t *tokens, *lengths;
   const float *u, *E;
-  int64_t u_bs, E_bs, tok_bs;
   int64_t *out, *accepted;
-  int B, N, V, chunk, n_chunk;
+  int B, N, V;
   double it;                      // 1 / T
   float c;
+  // split form
+  int chunk, n_chunk;             // of the rows' sums
+  int race_chunk, n_race;         // of the draw
   MaxSumD* parts;                 // [B * (2 N + 1)][n_chunk]: target rows first, then draft rows
-  struct VerifyBest* best;        // [B][n_chunk]
+  struct VerifyBest* best;        // [B][n_race]
 };
 
-// the running argmax of the race: score, bounds of the exact score, the largest upper bound of any other, where
+// the running argmax of the draw: score, bounds of the exact score, the largest upper bound of any other, where
 struct VerifyBest {
   float score, lower, upper, other;
   int at;
@@ -49,70 +49,45 @@ __device__ __forceinline__ void best_merge(VerifyBest& a, const VerifyBest& b) {
 
 template <class D>
 __device__ __forceinline__ const typename D::store* target_row(const VerifyArgs& A, int b, int i) {
-  return (const typename D::store*)A.target + b * A.tr.bs + i * A.tr.rs;
+  return (const typename D::store*)A.target + b * A.t_bs + i * A.t_rs;
 }
 template <class D>
 __device__ __forceinline__ const typename D::store* draft_row(const VerifyArgs& A, int b, int i) {
-  return (const typename D::store*)A.draft + b * A.qr.bs + i * A.qr.rs;
+  return (const typename D::store*)A.draft + b * A.q_bs + i * A.q_rs;
 }
 __device__ __forceinline__ int draft_length(const VerifyArgs& A, int b) {
   if (!A.lengths) return A.N;
   const int64_t n = A.lengths[b];
   return n < 0 ? 0 : n > A.N ? A.N : (int)n;
 }
-
-// ---- (max, sum of exponentials) of every row that can be asked for ------------------------------------------------------
-template <class D>
-__global__ __launch_bounds__(256) void nast_verify_lse_kernel(VerifyArgs A) {
-  __shared__ double red[8];
-  const int row = blockIdx.x / A.n_chunk, lo = (int)(blockIdx.x % A.n_chunk) * A.chunk, hi = min(A.V, lo + A.chunk);
-  const int n_target = A.B * (A.N + 1);
-  const bool is_target = row < n_target;
-  const int b = is_target ? row / (A.N + 1) : (row - n_target) / A.N, i = is_target ? row % (A.N + 1) : (row - n_target) % A.N;
-  const int len = draft_length(A, b);
-  if (is_target ? i > len : i >= len) return;
-  const typename D::store* p = is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i);
-  const MaxSum a = span_max_sum<D, 256>(p, lo, hi, A.c);
-  const MaxSumD t = block_max_sum<256>(a, A.c, red);
-  if (threadIdx.x == 0) A.parts[blockIdx.x] = t;
-}
-
-// a row's pair; a row without a distribution (a NaN, a +inf, nothing but -inf) has s = 0
-__device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
-  const MaxSumD* q = A.parts + (int64_t)row * A.n_chunk;
-  MaxSumD t = q[0];
-  for (int i = 1; i < A.n_chunk; ++i) {
-    const MaxSumD o = q[i];
-    const double m = fmax(t.m, o.m);
-    t.s = t.s * exp((t.m - m) * A.it) + o.s * exp((o.m - m) * A.it);
-    t.m = m;
-  }
+// a row without a distribution (a NaN, a +inf, nothing but -inf) has s = 0
+__device__ __forceinline__ MaxSumD proper(MaxSumD t) {
   if (!(t.s > 0 && t.m <= (double)FLT_MAX)) t.s = 0;
   return t;
 }
 
-// the same sum in double, by the whole workgroup of 256
-template <class D>
+// a row's sum in double, by the whole workgroup
+template <class D, int NT>
 __device__ double row_sum_exact(const VerifyArgs& A, const typename D::store* p, double m, double* red) {
   double s = 0;
-  for (int e = threadIdx.x; e < A.V; e += 256) s += exp(((double)D::get(p[e]) - m) * A.it);
+  for (int e = threadIdx.x; e < A.V; e += NT) s += exp(((double)D::get(p[e]) - m) * A.it);
   s = wave_sum_d(s);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  s = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) s += red[i];
+  return s;
 }
 
-struct VerifyDecision {
-  int accepted, len;
-};
 // p_i(d_i) and q_i(d_i); a token that is not one, or a row without a distribution: 0
 struct VerifyPair {
   double p, q;
 };
 template <class D>
 __device__ __forceinline__ VerifyPair drafted(const VerifyArgs& A, int b, int i, const MaxSumD& p, const MaxSumD& q) {
-  const int64_t d = A.tokens[b * A.tok_bs + i];
+  const int64_t d = A.tokens[(int64_t)b * A.N + i];
   if (d < 0 || d >= A.V || p.s == 0 || q.s == 0) return {0, 0};
   VerifyPair r;
   r.p = exp(((double)D::get(target_row<D>(A, b, i)[d]) - p.m) * A.it) / p.s;
@@ -120,78 +95,76 @@ __device__ __forceinline__ VerifyPair drafted(const VerifyArgs& A, int b, int i,
   return r;
 }
 __device__ __forceinline__ bool stands(const VerifyPair& r, float u) { return r.q > 0 && (double)u * r.q < r.p; }
-
-// How many drafts of sequence b stand, by the whole workgroup.  Each wavefront does the same: lane = position.
-template <class D>
-__device__ VerifyDecision decide(const VerifyArgs& A, int b, double* red) {
-  const int len = draft_length(A, b), lane = threadIdx.x & 63;
-  const int q0 = A.B * (A.N + 1) + b * A.N;
-  for (int base = 0; base < len; base += 64) {
-    const int i = base + lane;
-    bool ok = true, near = false;
-    if (i < len) {
-      const MaxSumD p = row_pair(A, b * (A.N + 1) + i);
-      const MaxSumD q = A.draft ? row_pair(A, q0 + i) : MaxSumD{0, 1};
-      const VerifyPair r = drafted<D>(A, b, i, p, q);
-      const float u = A.u[b * A.u_bs + i];
-      ok = stands(r, u);
-      near = r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= VERIFY_REL * r.p;
-    }
-    uint64_t no = __ballot(!ok), close = __ballot(near);
-    while (close) {
-      const int at = __ffsll((unsigned long long)close) - 1;
-      if (no & ((1ull << at) - 1)) break;                  // a clear refusal comes first
-      close &= close - 1;
-      const int j = base + at;
-      MaxSumD p = row_pair(A, b * (A.N + 1) + j), q = A.draft ? row_pair(A, q0 + j) : MaxSumD{0, 1};
-      p.s = row_sum_exact<D>(A, target_row<D>(A, b, j), p.m, red);
-      if (A.draft) q.s = row_sum_exact<D>(A, draft_row<D>(A, b, j), q.m, red);
-      const bool yes = stands(drafted<D>(A, b, j, p, q), A.u[b * A.u_bs + j]);
-      no = yes ? no & ~(1ull << at) : no | (1ull << at);
-    }
-    if (no) return {base + __ffsll((unsigned long long)no) - 1, len};
-  }
-  return {len, len};
+__device__ __forceinline__ bool too_close(const VerifyPair& r, float u) {
+  return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= 2 * VERIFY_REL * r.p;
+}
+// the same decision with sums in double, by the whole workgroup
+template <class D, int NT>
+__device__ bool stands_exact(const VerifyArgs& A, int b, int i, MaxSumD p, MaxSumD q, double* red) {
+  p.s = row_sum_exact<D, NT>(A, target_row<D>(A, b, i), p.m, red);
+  if (A.draft) q.s = row_sum_exact<D, NT>(A, draft_row<D>(A, b, i), q.m, red);
+  return stands(drafted<D>(A, b, i, p, q), A.u[(int64_t)b * A.N + i]);
 }
 
-// the row drawn from: p = exp((z - m) / T) / s, less q where the draft at that place was refused
+// What the token at place `place` is drawn from: p = exp((z - m) / T) / s, less q where the draft at that place was refused
 struct VerifyDraw {
   MaxSumD p, q;
-  int64_t one;                    // the refused draft's token where it came without probabilities, else -1
+  int place, one;                 // one: the refused draft's token where it came without probabilities, else -1
   bool minus_q;
 };
-template <class D>
-__device__ __forceinline__ VerifyDraw draw_of(const VerifyArgs& A, int b, const VerifyDecision& d) {
-  VerifyDraw w;
-  w.p = row_pair(A, b * (A.N + 1) + d.accepted);
-  w.q = {0, 0};
-  w.one = -1;
-  w.minus_q = false;
-  if (d.accepted < d.len) {
+__device__ __forceinline__ VerifyDraw draw_of(const VerifyArgs& A, int b, int place, int len, const MaxSumD& p, const MaxSumD& q) {
+  VerifyDraw w{p, q, place, -1, false};
+  if (place < len) {
     if (A.draft) {
-      w.q = row_pair(A, A.B * (A.N + 1) + b * A.N + d.accepted);
-      w.minus_q = w.q.s > 0;
+      w.minus_q = q.s > 0;
     } else {
-      w.one = A.tokens[b * A.tok_bs + d.accepted];
+      const int64_t d = A.tokens[(int64_t)b * A.N + place];
+      w.one = d >= 0 && d < A.V ? (int)d : -1;
     }
   }
   return w;
 }
 
-// argmax of w / E over [lo, hi) in fp32 with error bounds, by the whole workgroup
-template <class D>
-__device__ VerifyBest race(const VerifyArgs& A, int b, int place, const VerifyDraw& w, int lo, int hi, VerifyBest* lds) {
+// Argmax of w / E over [lo, hi) in fp32 with error bounds, by the whole workgroup.  An element is looked at closer only where its upper
+// bound exceeds the best lower bound that its wavefront has seen.
+template <class D, int NT>
+__device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int lo, int hi, VerifyBest* lds) {
   VerifyBest a{0.f, 0.f, 0.f, 0.f, 0x7fffffff};
   if (w.p.s > 0) {
-    const typename D::store* p = target_row<D>(A, b, place);
-    const typename D::store* q = w.minus_q ? draft_row<D>(A, b, place) : nullptr;
-    const float* E = A.E + b * A.E_bs;
-    const float pm = (float)w.p.m, ps = (float)(1.0 / w.p.s), qm = (float)w.q.m, qs = w.minus_q ? (float)(1.0 / w.q.s) : 0.f;
-    for (int e = lo + threadIdx.x; e < hi; e += 256) {
-      if (e == w.one) continue;
-      const float pv = exp_t(D::get(p[e]) - pm, A.c) * ps, qv = q ? exp_t(D::get(q[e]) - qm, A.c) * qs : 0.f;
-      const float inv = 1.0f / E[e], d = pv - qv, err = (pv + qv) * (float)VERIFY_REL + 1e-37f;
-      best_merge(a, {d * inv, (d - err) * inv, (d + err) * inv, 0.f, e});
+    const typename D::store* p = target_row<D>(A, b, w.place);
+    const typename D::store* q = w.minus_q ? draft_row<D>(A, b, w.place) : nullptr;
+    const float* E = A.E + (int64_t)b * A.V;
+    const float pm = (float)w.p.m, qm = (float)w.q.m, ps = -(float)log2(w.p.s), qs = w.minus_q ? -(float)log2(w.q.s) : 0.f;
+    float seen = 0.f;
+    auto look = [&](float zp, float zq, float en, int e) {
+      const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(zp - pm, A.c, ps));
+      const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(zq - qm, A.c, qs)) : 0.f;
+      const float inv = __builtin_amdgcn_rcpf(en), d = pv - qv, err = __builtin_fmaf(pv + qv, VERIFY_REL, 1e-37f), upper = (d + err) * inv;
+      if (upper > seen && e != w.one) best_merge(a, {d * inv, (d - err) * inv, upper, 0.f, e});
+    };
+    const RowSpan16<D> rs(p, lo, hi);
+    const int e = rs.edge(threadIdx.x);
+    if (e >= 0) look(D::get(p[e]), q ? D::get(q[e]) : 0.f, E[e], e);
+    constexpr int U = 2, W = D::EPV / 4;                        // W: vectors of draws to one of logits
+    for (int b0 = 0; b0 < rs.n; b0 += NT * U) {
+      RowVec<D> pv[U], qv[U];
+      RowVec<RowF32> ev[U][W];
+      seen = wave_max(fmaxf(seen, a.lower));                    // (every lane takes part)
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int at = rs.elem(min(b0 + NT * i + (int)threadIdx.x, rs.n - 1));
+        pv[i] = vec_load<D>(p + at);
+        qv[i] = vec_load_any<D>((q ? q : p) + at);
+#pragma unroll
+        for (int j = 0; j < W; ++j) ev[i][j] = vec_load_any<RowF32>(E + at + 4 * j);
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int s = b0 + NT * i + (int)threadIdx.x;
+        if (s < rs.n)
+#pragma unroll
+          for (int j = 0; j < D::EPV; ++j) look(pv[i].get(j), qv[i].get(j), ev[i][j / 4].get(j % 4), rs.elem(s) + j);
+      }
     }
   }
 #pragma unroll
@@ -204,33 +177,32 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, int place, const VerifyDr
     x.at = __shfl_xor(a.at, o, 64);
     best_merge(a, x);
   }
-  const int wv = threadIdx.x >> 6;
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) lds[wv] = a;
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
   __syncthreads();
   VerifyBest r = lds[0];
-  for (int i = 1; i < 4; ++i) best_merge(r, lds[i]);
+  for (int i = 1; i < NT / 64; ++i) best_merge(r, lds[i]);
   return r;
 }
 
 // The draw in double, ties to the lowest id.  Where nothing is left of p - q (rounding, u >= 1) it is made from p.
-template <class D>
-__device__ int race_exact(const VerifyArgs& A, int b, int place, VerifyDraw w, double* red, int* ired) {
+template <class D, int NT>
+__device__ int race_exact(const VerifyArgs& A, int b, const VerifyDraw& w, double* red, int* ired) {
   if (w.p.s == 0) return -1;
-  const typename D::store* p = target_row<D>(A, b, place);
-  const typename D::store* q = w.minus_q ? draft_row<D>(A, b, place) : nullptr;
-  const double ps = row_sum_exact<D>(A, p, w.p.m, red), qs = q ? row_sum_exact<D>(A, q, w.q.m, red) : 1;
+  const typename D::store* p = target_row<D>(A, b, w.place);
+  const typename D::store* q = w.minus_q ? draft_row<D>(A, b, w.place) : nullptr;
+  const double ps = row_sum_exact<D, NT>(A, p, w.p.m, red), qs = q ? row_sum_exact<D, NT>(A, q, w.q.m, red) : 1;
   for (int whole = 0; whole < 2; ++whole) {
     double best = 0;
     int at = 0x7fffffff;
-    for (int e = threadIdx.x; e < A.V; e += 256) {
+    for (int e = threadIdx.x; e < A.V; e += NT) {
       double v = exp(((double)D::get(p[e]) - w.p.m) * A.it) / ps;
       if (!whole) {
         if (q) v -= exp(((double)D::get(q[e]) - w.q.m) * A.it) / qs;
         if (e == w.one) v = 0;
       }
       if (!(v > 0)) continue;
-      const double score = v / (double)A.E[b * A.E_bs + e];
+      const double score = v / (double)A.E[(int64_t)b * A.V + e];
       if (score > best) {
         best = score;
         at = e;
@@ -251,7 +223,7 @@ __device__ int race_exact(const VerifyArgs& A, int b, int place, VerifyDraw w, d
       ired[threadIdx.x >> 6] = at;
     }
     __syncthreads();
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < NT / 64; ++i)
       if (red[i] > best || (red[i] == best && ired[i] < at)) {
         best = red[i];
         at = ired[i];
@@ -262,16 +234,127 @@ __device__ int race_exact(const VerifyArgs& A, int b, int place, VerifyDraw w, d
   return -1;
 }
 
+// the end of a sequence, by the whole workgroup
+template <class D, int NT>
+__device__ void finish(const VerifyArgs& A, int b, const VerifyDraw& w, const VerifyBest& a, double* red, int* ired) {
+  const int token = a.lower > a.other ? a.at : race_exact<D, NT>(A, b, w, red, ired);
+  for (int i = threadIdx.x; i <= A.N; i += NT)
+    A.out[(int64_t)b * (A.N + 1) + i] = i < w.place ? A.tokens[(int64_t)b * A.N + i] : i == w.place ? token : -1;
+  if (threadIdx.x == 0) A.accepted[b] = w.place;
+}
+
+// ---------------------------------------------------------------------------------------------
+// One workgroup per sequence, place after place: no row behind a refused draft is read, one launch, no workspace.  For batches that
+// fill the card.
+// ---------------------------------------------------------------------------------------------
+template <class D, int NT>
+__global__ __launch_bounds__(NT) void nast_verify_whole_kernel(VerifyArgs A) {
+  __shared__ double red[2 * NT / 64];
+  __shared__ int ired[NT / 64];
+  __shared__ VerifyBest lds[NT / 64];
+  const int b = blockIdx.x, len = draft_length(A, b);
+  MaxSumD p, q{0, 1};
+  int i = 0;
+  for (;; ++i) {
+    const MaxSum mine = span_max_sum<D, NT, 8>(target_row<D>(A, b, i), 0, A.V, A.c);
+    if (i < len && A.draft) {
+      const MaxSum other = span_max_sum<D, NT, 8>(draft_row<D>(A, b, i), 0, A.V, A.c);
+      q = proper(block_max_sum<NT>(other, A.c, red));
+    }
+    p = proper(block_max_sum<NT>(mine, A.c, red));
+    if (i == len) break;
+    const VerifyPair r = drafted<D>(A, b, i, p, q);
+    const float u = A.u[(int64_t)b * A.N + i];
+    if (!(too_close(r, u) ? stands_exact<D, NT>(A, b, i, p, q, red) : stands(r, u))) break;
+  }
+  const VerifyDraw w = draw_of(A, b, i, len, p, q);
+  const VerifyBest a = race<D, NT>(A, b, w, 0, A.V, lds);
+  finish<D, NT>(A, b, w, a, red, ired);
+}
+
+// ---------------------------------------------------------------------------------------------
+// All rows at once, in chunks; then the draw, each workgroup finding the place for itself: in one workgroup a sequence, or in chunks that
+// a third launch joins.  For small batches.
+// ---------------------------------------------------------------------------------------------
 template <class D>
-__global__ __launch_bounds__(256) void nast_verify_race_kernel(VerifyArgs A) {
-  __shared__ double red[4];
-  __shared__ VerifyBest lds[4];
-  const int b = blockIdx.x / A.n_chunk, lo = (int)(blockIdx.x % A.n_chunk) * A.chunk, hi = min(A.V, lo + A.chunk);
-  const VerifyDecision d = decide<D>(A, b, red);
-  const VerifyBest a = race<D>(A, b, d.accepted, draw_of<D>(A, b, d), lo, hi, lds);
-  if (threadIdx.x == 0) {
+__global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A) {
+  __shared__ double red[8];
+  const int row = blockIdx.x / A.n_chunk, ch = blockIdx.x % A.n_chunk, lo = ch * A.chunk, hi = min(A.V, lo + A.chunk);
+  const int n_target = A.B * (A.N + 1);
+  const bool is_target = row < n_target;
+  const int b = is_target ? row / (A.N + 1) : (row - n_target) / A.N, i = is_target ? row % (A.N + 1) : (row - n_target) % A.N;
+  const int len = draft_length(A, b);
+  if (is_target ? i > len : i >= len) return;
+  const MaxSum a = span_max_sum<D, 256>(is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i), lo, hi, A.c);
+  const MaxSumD t = block_max_sum<256>(a, A.c, red);
+  if (threadIdx.x == 0) A.parts[blockIdx.x] = t;
+}
+
+__device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
+  const MaxSumD* q = A.parts + (int64_t)row * A.n_chunk;
+  MaxSumD t = q[0];
+  for (int i = 1; i < A.n_chunk; i += 4) {                     // four loads in flight
+    MaxSumD o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = q[min(i + j, A.n_chunk - 1)];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j >= A.n_chunk) break;
+      const double m = fmax(t.m, o[j].m);
+      t.s = t.s * (double)exp_t((float)(t.m - m), A.c) + o[j].s * (double)exp_t((float)(o[j].m - m), A.c);
+      t.m = m;
+    }
+  }
+  return proper(t);
+}
+
+// How many drafts of sequence b stand, by the whole workgroup.  Each wavefront does the same: lane = place.
+template <class D, int NT>
+__device__ int places(const VerifyArgs& A, int b, int len, double* red) {
+  const int lane = threadIdx.x & 63, p0 = b * (A.N + 1), q0 = A.B * (A.N + 1) + b * A.N;
+  for (int base = 0; base < len; base += 64) {
+    const int i = base + lane;
+    bool ok = true, near = false;
+    if (i < len) {
+      const VerifyPair r = drafted<D>(A, b, i, row_pair(A, p0 + i), A.draft ? row_pair(A, q0 + i) : MaxSumD{0, 1});
+      const float u = A.u[(int64_t)b * A.N + i];
+      ok = stands(r, u);
+      near = too_close(r, u);
+    }
+    uint64_t no = __ballot(!ok), close = __ballot(near);
+    while (close) {
+      const int at = __ffsll((unsigned long long)close) - 1;
+      if (no & ((1ull << at) - 1)) break;                  // a clear refusal comes first
+      close &= close - 1;
+      const int j = base + at;
+      const bool yes = stands_exact<D, NT>(A, b, j, row_pair(A, p0 + j), A.draft ? row_pair(A, q0 + j) : MaxSumD{0, 1}, red);
+      no = yes ? no & ~(1ull << at) : no | (1ull << at);
+    }
+    if (no) return base + __ffsll((unsigned long long)no) - 1;
+  }
+  return len;
+}
+
+template <class D>
+__device__ __forceinline__ VerifyDraw draw_at(const VerifyArgs& A, int b, int place, int len) {
+  return draw_of(A, b, place, len, row_pair(A, b * (A.N + 1) + place),
+                 A.draft && place < len ? row_pair(A, A.B * (A.N + 1) + b * A.N + place) : MaxSumD{0, 0});
+}
+
+template <class D, int NT>
+__global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
+  __shared__ double red[NT / 64];
+  __shared__ int ired[NT / 64];
+  __shared__ VerifyBest lds[NT / 64];
+  const int b = blockIdx.x / A.n_race, lo = (int)(blockIdx.x % A.n_race) * A.race_chunk, hi = min(A.V, lo + A.race_chunk);
+  const int len = draft_length(A, b), place = places<D, NT>(A, b, len, red);
+  const VerifyDraw w = draw_at<D>(A, b, place, len);
+  const VerifyBest a = race<D, NT>(A, b, w, lo, hi, lds);
+  if (A.n_race == 1) {
+    finish<D, NT>(A, b, w, a, red, ired);
+  } else if (threadIdx.x == 0) {
     A.best[blockIdx.x] = a;
-    if (lo == 0) A.accepted[b] = d.accepted;
+    if (lo == 0) A.accepted[b] = place;
   }
 }
 
@@ -279,21 +362,39 @@ template <class D>
 __global__ __launch_bounds__(256) void nast_verify_join_kernel(VerifyArgs A) {
   __shared__ double red[4];
   __shared__ int ired[4];
-  const int b = blockIdx.x;
-  const VerifyDecision d{(int)A.accepted[b], draft_length(A, b)};
-  VerifyBest a = A.best[(int64_t)b * A.n_chunk];
-  for (int i = 1; i < A.n_chunk; ++i) best_merge(a, A.best[(int64_t)b * A.n_chunk + i]);
-  int token = a.at;
-  if (!(a.lower > a.other)) token = race_exact<D>(A, b, d.accepted, draw_of<D>(A, b, d), red, ired);
-  for (int i = threadIdx.x; i <= A.N; i += 256)
-    A.out[(int64_t)b * (A.N + 1) + i] = i < d.accepted ? A.tokens[b * A.tok_bs + i] : i == d.accepted ? token : -1;
+  const int b = blockIdx.x, len = draft_length(A, b), place = (int)A.accepted[b];
+  VerifyBest a = A.best[(int64_t)b * A.n_race];
+  for (int i = 1; i < A.n_race; ++i) best_merge(a, A.best[(int64_t)b * A.n_race + i]);
+  VerifyDraw w{};
+  w.place = place;
+  if (!(a.lower > a.other)) w = draw_at<D>(A, b, place, len);
+  finish<D, 256>(A, b, w, a, red, ired);
 }
 
-static int verify_chunks(int V) { return (V + VERIFY_CHUNK - 1) / VERIFY_CHUNK; }
+static bool verify_whole(int B) { return B >= 64; }
+
+static void verify_plan(VerifyArgs& A, int dtype) {
+  const int most = 1 << 15;
+  A.n_chunk = row_chunks(A.B * (A.draft ? 2 * A.N + 1 : A.N + 1), A.V, most, 1 << 13);
+  A.chunk = (A.V + A.n_chunk - 1) / A.n_chunk;
+  A.n_race = A.V <= 1 << 16 ? 1 : row_chunks(A.B, A.V, most, 1 << 13);
+  A.race_chunk = (A.V + A.n_race - 1) / A.n_race;
+}
 
 extern "C" int64_t nast_verify_draft_workspace_bytes(int B, int N, int V, int dtype) {
-  const int64_t n = verify_chunks(V);
-  return ((int64_t)B * (2 * N + 1) * (int64_t)sizeof(MaxSumD) + (int64_t)B * (int64_t)sizeof(VerifyBest)) * n;
+  if (B < 1 || N < 0 || N > VERIFY_MAX_DRAFTS || V < 1 || V > VERIFY_MAX_V || verify_whole(B)) return 0;
+  int64_t most = 0;
+  for (int draft = 0; draft < 2; ++draft) {                   // (with and without draft logits)
+    VerifyArgs A;
+    A.B = B;
+    A.N = N;
+    A.V = V;
+    A.draft = draft ? &A : nullptr;
+    verify_plan(A, dtype);
+    const int64_t n = (int64_t)B * (2 * N + 1) * A.n_chunk * (int64_t)sizeof(MaxSumD) + (int64_t)B * A.n_race * (int64_t)sizeof(VerifyBest);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t target_rs, const void* draft, int64_t draft_bs,
@@ -301,42 +402,50 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
                                  const int64_t* lengths, int64_t* out, int64_t* accepted, int B, int N, int V, double temp,
                                  void* workspace, void* stream) {
   NAST_REQUIRE(row_dtype_ok(dtype), "nast_verify_draft: unknown dtype %d", dtype);
-  NAST_REQUIRE(B >= 0 && N >= 0 && N <= VERIFY_MAX_DRAFTS && V >= 1 && V < (1 << 24), "nast_verify_draft: bad sizes B=%d N=%d V=%d", B, N, V);
+  NAST_REQUIRE(B >= 0 && B < (1 << 20) && N >= 0 && N <= VERIFY_MAX_DRAFTS && V >= 1 && V <= VERIFY_MAX_V,
+               "nast_verify_draft: bad sizes B=%d N=%d V=%d", B, N, V);
   NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_verify_draft: temperature must be > 0 and finite");
   if (B == 0) return NAST_OK;
-  NAST_REQUIRE(target && E && out && accepted && workspace && (N == 0 || (tokens && u)), "nast_verify_draft: NULL pointer");
+  NAST_REQUIRE(target && E && out && accepted && (verify_whole(B) || workspace) && (N == 0 || (tokens && u)),
+               "nast_verify_draft: NULL pointer");
   NAST_REQUIRE(row_aligned(target, dtype) && row_aligned(draft, dtype), "nast_verify_draft: misaligned pointer");
   VerifyArgs A;
   A.target = target;
   A.draft = N ? draft : nullptr;
-  A.tr = {target_bs, target_rs};
-  A.qr = {draft_bs, draft_rs};
+  A.t_bs = target_bs;
+  A.t_rs = target_rs;
+  A.q_bs = draft_bs;
+  A.q_rs = draft_rs;
   A.tokens = tokens;
   A.lengths = lengths;
   A.u = u;
   A.E = E;
-  A.u_bs = A.tok_bs = N;
-  A.E_bs = V;
   A.out = out;
   A.accepted = accepted;
   A.B = B;
   A.N = N;
   A.V = V;
-  A.chunk = VERIFY_CHUNK;
-  A.n_chunk = verify_chunks(V);
   A.it = 1.0 / temp;
   A.c = exp_scale(temp);
-  A.parts = (MaxSumD*)workspace;
-  const int64_t rows = (int64_t)B * (A.draft ? 2 * N + 1 : N + 1);
-  A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
-  NAST_REQUIRE(rows * A.n_chunk < (1 << 24), "nast_verify_draft: too many rows (%lld)", (long long)rows);
   hipStream_t s = (hipStream_t)stream;
+  const int rows = B * (A.draft ? 2 * N + 1 : N + 1);
   nast_prof_before(2, s);
-  NAST_ROW_DTYPE(dtype, {
-    hipLaunchKernelGGL((nast_verify_lse_kernel<D>), dim3((unsigned)(rows * A.n_chunk)), dim3(256), 0, s, A);
-    hipLaunchKernelGGL((nast_verify_race_kernel<D>), dim3(B * A.n_chunk), dim3(256), 0, s, A);
-    hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(256), 0, s, A);
-  });
+  if (verify_whole(B)) {
+    NAST_ROW_DTYPE(dtype, hipLaunchKernelGGL((nast_verify_whole_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A));
+  } else {
+    verify_plan(A, dtype);
+    A.parts = (MaxSumD*)workspace;
+    A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
+    NAST_ROW_DTYPE(dtype, {
+      hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(rows * A.n_chunk), dim3(256), 0, s, A);
+      if (A.n_race == 1) {
+        hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
+      } else {
+        hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B * A.n_race), dim3(256), 0, s, A);
+        hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(256), 0, s, A);
+      }
+    });
+  }
   nast_prof_after(2, s, (double)V * (row_size(dtype) * (double)rows + 4.0 * B));
   NAST_CHECK_LAUNCH("nast_verify_draft");
   return NAST_OK;

@@ -101,7 +101,8 @@ def test_c_entries_refuse():
     refused(*ver(tok=None), match="NULL")
     refused(*ver(ws=None), match="NULL")
     refused(*ver(q=P + 2), match="misaligned")
-    refused(*ver(B=1 << 20, N=15), match="too many rows")
+    refused(*ver(B=1 << 20, N=15), match="bad sizes")
+    refused(*ver(V=(1 << 20) + 1), match="bad sizes")
     for name, args in (("nast_top_logits_workspace_bytes", (2, 8, 3, 0)), ("nast_top_distill_workspace_bytes", (2, 8, 0)),
                        ("nast_verify_draft_workspace_bytes", (2, 3, 8, 0))):
         assert getattr(_lib.load(), name)(*args) >= 0
