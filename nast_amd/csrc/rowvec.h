@@ -97,9 +97,12 @@ __device__ __forceinline__ float exp_t(float t, float c) { return __builtin_amdg
 
 // Sum of exponentials relative to a maximum.  The maximum starts at the lowest finite value, so that no -inf is subtracted from
 // -inf: a row of -inf ends with s = 0 (log-sum-exp -inf), a row of the type's lowest value counts as any other row.  A NaN or
-// +inf among the elements leaves s = NaN.  s is fp32 inside a thread (at most a few hundred terms), double across threads.
+// +inf among the elements leaves s = NaN.  Vectors are summed in fp32 (at most 32 terms), everything from there in double.
+// What s is off by, relative: 4e-6.  An exponential 2^-a has 3 roundings of its argument, 1.24e-7 * a, and the instruction's 1.2e-7;
+// weighted by the exponentials themselves a is log2(V) <= 20 on average at most (entropy); 12 roundings of a sum add 7e-7.
 struct MaxSum {
-  float m, s;
+  float m;
+  double s;
 };
 // U vectors at a time: one comparison with the running maximum and at most one rescaling for all of them
 template <class D, int U>
@@ -110,23 +113,25 @@ __device__ __forceinline__ void fold(MaxSum& a, const RowVec<D> (&v)[U], float c
 #pragma unroll
     for (int i = 0; i < D::EPV; ++i) top = fmaxf(top, v[u].get(i));
   if (top > a.m) {
-    a.s *= exp_t(a.m - top, c);
+    a.s *= (double)exp_t(a.m - top, c);
     a.m = top;
   }
+  float all = 0.f;
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < D::EPV; ++i) s += exp_t(v[u].get(i) - a.m, c);
-    a.s += s;
+    all += s;
   }
+  a.s += (double)all;
 }
 __device__ __forceinline__ void fold_one(MaxSum& a, float f, float c) {
   if (f > a.m) {
-    a.s *= exp_t(a.m - f, c);
+    a.s *= (double)exp_t(a.m - f, c);
     a.m = f;
   }
-  a.s += exp_t(f - a.m, c);
+  a.s += (double)exp_t(f - a.m, c);
 }
 
 // The slots of a span in batches of U vectors a thread: full(v, first slot) for a batch that every thread has whole, part(v, slot) for
@@ -156,7 +161,7 @@ __device__ __forceinline__ MaxSum span_max_sum(const typename D::store* p, int l
   const RowSpan16<D> rs(p, lo, hi);
   const int e = rs.edge(threadIdx.x);
   const typename D::store edge = p[e >= 0 ? e : lo];
-  MaxSum a{-FLT_MAX, 0.f};
+  MaxSum a{-FLT_MAX, 0.0};
   for_slots<D, NT, U>(rs, [&](int s) { return rs.load(p, s); }, [&](const RowVec<D>(&v)[U], int) { fold<D, U>(a, v, c); },
                       [&](const RowVec<D>& v, int) {
                         const RowVec<D> one[1] = {v};
@@ -183,7 +188,7 @@ __device__ __forceinline__ double wave_max_d(double v) {
 template <int NT>
 __device__ __forceinline__ MaxSumD block_max_sum(MaxSum a, float c, double* red) {
   const float wm = wave_max(a.m);
-  const double ws = wave_sum_d((double)(a.s * exp_t(a.m - wm, c)));
+  const double ws = wave_sum_d(a.s * (double)exp_t(a.m - wm, c));
   const int w = threadIdx.x >> 6;
   __syncthreads();
   if ((threadIdx.x & 63) == 0) {

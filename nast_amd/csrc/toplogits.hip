@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
   const int64_t r = block / n_chunk;
   const int lo = (int)(block % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
-  MaxSum a{-FLT_MAX, 0.f};
+  MaxSum a{-FLT_MAX, 0.0};
   SlotSums q;
   if (!SPLIT) q = slot_sums<D, 256, TAIL>(r, p, t, t_dtype, idx, K, lse_t, V, it, ids, red);
   if (!TAIL) {
@@ -776,7 +776,7 @@ static int distill_check(const char* name, int dtype, int t_dtype, int K, int ro
   return NAST_OK;
 }
 // One workgroup reads a whole row where there are rows enough to fill the card (512: two workgroups a compute unit); a chunk has at
-// least 16 Ki elements and at most 2^15 vectors: a thread's fp32 sum has 128 of them, the membership bits take 40 KB.
+// least 16 Ki elements and at most 2^15 vectors (the membership bits of 2^18 elements take 40 KB).
 struct DistillPlan {
   int n, chunk;
 };

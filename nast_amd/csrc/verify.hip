@@ -11,9 +11,10 @@
 
 #define VERIFY_MAX_V (1 << 20)
 #define VERIFY_MAX_DRAFTS 1024
-// What the fp32 probabilities here are off by, relative: sums of exponentials 1.6e-5 (at most 256 vectors of 4 a thread, one rounding
-// each), exponents of magnitude up to 126 three roundings each, 1.6e-5, and the instructions' own.
-#define VERIFY_REL 4e-5f
+// What the fp32 probabilities of the draw are off by, relative: the row's sum 4e-6 (see MaxSum), an exponent of -a before and of up to
+// a + 20 after the sum's logarithm is added ln 2 * 2^-24 * (4 a + 40), the instruction 1.2e-7.
+#define VERIFY_REL 6e-6f
+#define VERIFY_REL_EXP 2e-7f
 
 struct VerifyArgs {
   const void *target, *draft;     // draft NULL: no probabilities
@@ -24,7 +25,6 @@ struct VerifyArgs {
   int B, N, V;
   double it;                      // 1 / T
   float c;
-  // split form
   int chunk, n_chunk;             // of the rows' sums
   int race_chunk, n_race;         // of the draw
   MaxSumD* parts;                 // [B * (2 N + 1)][n_chunk]: target rows first, then draft rows
@@ -96,7 +96,7 @@ __device__ __forceinline__ VerifyPair drafted(const VerifyArgs& A, int b, int i,
 }
 __device__ __forceinline__ bool stands(const VerifyPair& r, float u) { return r.q > 0 && (double)u * r.q < r.p; }
 __device__ __forceinline__ bool too_close(const VerifyPair& r, float u) {
-  return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= 2 * VERIFY_REL * r.p;
+  return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= 1e-5 * r.p;   // (two sums)
 }
 // the same decision with sums in double, by the whole workgroup
 template <class D, int NT>
@@ -135,11 +135,15 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     const typename D::store* q = w.minus_q ? draft_row<D>(A, b, w.place) : nullptr;
     const float* E = A.E + (int64_t)b * A.V;
     const float pm = (float)w.p.m, qm = (float)w.q.m, ps = -(float)log2(w.p.s), qs = w.minus_q ? -(float)log2(w.q.s) : 0.f;
+    const float slope = -VERIFY_REL_EXP * A.c;
     float seen = 0.f;
     auto look = [&](float zp, float zq, float en, int e) {
-      const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(zp - pm, A.c, ps));
-      const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(zq - qm, A.c, qs)) : 0.f;
-      const float inv = __builtin_amdgcn_rcpf(en), d = pv - qv, err = __builtin_fmaf(pv + qv, VERIFY_REL, 1e-37f), upper = (d + err) * inv;
+      const float tp = zp - pm, tq = zq - qm;
+      const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(tp, A.c, ps));
+      const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(tq, A.c, qs)) : 0.f;
+      const float d = pv - qv, inv = __builtin_amdgcn_rcpf(en);
+      const float err = 1e-37f + (pv * __builtin_fmaf(tp, slope, VERIFY_REL) + (q ? qv * __builtin_fmaf(tq, slope, VERIFY_REL) : 0.f));
+      const float upper = (d + err) * inv;
       if (upper > seen && e != w.one) best_merge(a, {d * inv, (d - err) * inv, upper, 0.f, e});
     };
     const RowSpan16<D> rs(p, lo, hi);
@@ -244,52 +248,10 @@ __device__ void finish(const VerifyArgs& A, int b, const VerifyDraw& w, const Ve
 }
 
 // ---------------------------------------------------------------------------------------------
-// One workgroup per sequence, place after place: no row behind a refused draft is read, one launch, no workspace.  For batches that
-// fill the card.
+// Rows are read in rounds of places, each a launch over (sequence, row, chunk); a round leaves out the sequences that a clear refusal of
+// an earlier one has ended, whose further rows nothing needs.  Then place and draw: by one workgroup a sequence, or the draw in chunks,
+// with a launch before it that finds the place and one behind it that joins them.
 // ---------------------------------------------------------------------------------------------
-template <class D, int NT>
-__global__ __launch_bounds__(NT) void nast_verify_whole_kernel(VerifyArgs A) {
-  __shared__ double red[2 * NT / 64];
-  __shared__ int ired[NT / 64];
-  __shared__ VerifyBest lds[NT / 64];
-  const int b = blockIdx.x, len = draft_length(A, b);
-  MaxSumD p, q{0, 1};
-  int i = 0;
-  for (;; ++i) {
-    const MaxSum mine = span_max_sum<D, NT, 8>(target_row<D>(A, b, i), 0, A.V, A.c);
-    if (i < len && A.draft) {
-      const MaxSum other = span_max_sum<D, NT, 8>(draft_row<D>(A, b, i), 0, A.V, A.c);
-      q = proper(block_max_sum<NT>(other, A.c, red));
-    }
-    p = proper(block_max_sum<NT>(mine, A.c, red));
-    if (i == len) break;
-    const VerifyPair r = drafted<D>(A, b, i, p, q);
-    const float u = A.u[(int64_t)b * A.N + i];
-    if (!(too_close(r, u) ? stands_exact<D, NT>(A, b, i, p, q, red) : stands(r, u))) break;
-  }
-  const VerifyDraw w = draw_of(A, b, i, len, p, q);
-  const VerifyBest a = race<D, NT>(A, b, w, 0, A.V, lds);
-  finish<D, NT>(A, b, w, a, red, ired);
-}
-
-// ---------------------------------------------------------------------------------------------
-// All rows at once, in chunks; then the draw, each workgroup finding the place for itself: in one workgroup a sequence, or in chunks that
-// a third launch joins.  For small batches.
-// ---------------------------------------------------------------------------------------------
-template <class D>
-__global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A) {
-  __shared__ double red[8];
-  const int row = blockIdx.x / A.n_chunk, ch = blockIdx.x % A.n_chunk, lo = ch * A.chunk, hi = min(A.V, lo + A.chunk);
-  const int n_target = A.B * (A.N + 1);
-  const bool is_target = row < n_target;
-  const int b = is_target ? row / (A.N + 1) : (row - n_target) / A.N, i = is_target ? row % (A.N + 1) : (row - n_target) % A.N;
-  const int len = draft_length(A, b);
-  if (is_target ? i > len : i >= len) return;
-  const MaxSum a = span_max_sum<D, 256>(is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i), lo, hi, A.c);
-  const MaxSumD t = block_max_sum<256>(a, A.c, red);
-  if (threadIdx.x == 0) A.parts[blockIdx.x] = t;
-}
-
 __device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
   const MaxSumD* q = A.parts + (int64_t)row * A.n_chunk;
   MaxSumD t = q[0];
@@ -308,15 +270,50 @@ __device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
   return proper(t);
 }
 
-// How many drafts of sequence b stand, by the whole workgroup.  Each wavefront does the same: lane = place.
+// the draft at place i of sequence b, from the rows' sums
+template <class D>
+__device__ __forceinline__ VerifyPair drafted_at(const VerifyArgs& A, int b, int i) {
+  return drafted<D>(A, b, i, row_pair(A, b * (A.N + 1) + i), A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + i) : MaxSumD{0, 1});
+}
+
+template <class D>
+__global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A, int i0, int n_target, int n_draft) {
+  __shared__ double red[8];
+  __shared__ int over;
+  const int k = blockIdx.x / A.n_chunk, ch = blockIdx.x % A.n_chunk, lo = ch * A.chunk, hi = min(A.V, lo + A.chunk);
+  const int b = k / (n_target + n_draft), j = k % (n_target + n_draft), len = draft_length(A, b);
+  const bool is_target = j < n_target;
+  const int i = i0 + (is_target ? j : j - n_target);
+  if (is_target ? i > len : i >= len) return;
+  if (i0 > 0) {                                                // i0 <= len here
+    if (threadIdx.x < 64) {
+      bool ended = false;
+      for (int l = threadIdx.x; l < i0; l += 64) {
+        const VerifyPair r = drafted_at<D>(A, b, l);
+        const float u = A.u[(int64_t)b * A.N + l];
+        ended = ended || (!stands(r, u) && !too_close(r, u));
+      }
+      const uint64_t any = __ballot(ended);
+      if (threadIdx.x == 0) over = any != 0;
+    }
+    __syncthreads();
+    if (over) return;
+  }
+  const MaxSum a = span_max_sum<D, 256>(is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i), lo, hi, A.c);
+  const MaxSumD t = block_max_sum<256>(a, A.c, red);
+  if (threadIdx.x == 0) A.parts[(int64_t)(is_target ? b * (A.N + 1) + i : A.B * (A.N + 1) + b * A.N + i) * A.n_chunk + ch] = t;
+}
+
+// How many drafts of sequence b stand, by the whole workgroup.  Each wavefront does the same: lane = place.  (Sums behind a clear refusal
+// may never have been written; what is made of them is not looked at.)
 template <class D, int NT>
 __device__ int places(const VerifyArgs& A, int b, int len, double* red) {
-  const int lane = threadIdx.x & 63, p0 = b * (A.N + 1), q0 = A.B * (A.N + 1) + b * A.N;
+  const int lane = threadIdx.x & 63;
   for (int base = 0; base < len; base += 64) {
     const int i = base + lane;
     bool ok = true, near = false;
     if (i < len) {
-      const VerifyPair r = drafted<D>(A, b, i, row_pair(A, p0 + i), A.draft ? row_pair(A, q0 + i) : MaxSumD{0, 1});
+      const VerifyPair r = drafted_at<D>(A, b, i);
       const float u = A.u[(int64_t)b * A.N + i];
       ok = stands(r, u);
       near = too_close(r, u);
@@ -327,7 +324,8 @@ __device__ int places(const VerifyArgs& A, int b, int len, double* red) {
       if (no & ((1ull << at) - 1)) break;                  // a clear refusal comes first
       close &= close - 1;
       const int j = base + at;
-      const bool yes = stands_exact<D, NT>(A, b, j, row_pair(A, p0 + j), A.draft ? row_pair(A, q0 + j) : MaxSumD{0, 1}, red);
+      const MaxSumD p = row_pair(A, b * (A.N + 1) + j), q = A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + j) : MaxSumD{0, 1};
+      const bool yes = stands_exact<D, NT>(A, b, j, p, q, red);
       no = yes ? no & ~(1ull << at) : no | (1ull << at);
     }
     if (no) return base + __ffsll((unsigned long long)no) - 1;
@@ -347,42 +345,56 @@ __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
   __shared__ int ired[NT / 64];
   __shared__ VerifyBest lds[NT / 64];
   const int b = blockIdx.x / A.n_race, lo = (int)(blockIdx.x % A.n_race) * A.race_chunk, hi = min(A.V, lo + A.race_chunk);
-  const int len = draft_length(A, b), place = places<D, NT>(A, b, len, red);
+  const int len = draft_length(A, b), place = A.n_race == 1 ? places<D, NT>(A, b, len, red) : (int)A.accepted[b];
   const VerifyDraw w = draw_at<D>(A, b, place, len);
   const VerifyBest a = race<D, NT>(A, b, w, lo, hi, lds);
   if (A.n_race == 1) {
     finish<D, NT>(A, b, w, a, red, ired);
   } else if (threadIdx.x == 0) {
     A.best[blockIdx.x] = a;
-    if (lo == 0) A.accepted[b] = place;
   }
 }
 
+// (1024 threads in these two for the sums in double that they may have to make)
 template <class D>
-__global__ __launch_bounds__(256) void nast_verify_join_kernel(VerifyArgs A) {
-  __shared__ double red[4];
-  __shared__ int ired[4];
+__global__ __launch_bounds__(1024) void nast_verify_place_kernel(VerifyArgs A) {
+  __shared__ double red[16];
+  const int b = blockIdx.x, place = places<D, 1024>(A, b, draft_length(A, b), red);
+  if (threadIdx.x == 0) A.accepted[b] = place;
+}
+
+template <class D>
+__global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
+  __shared__ double red[16];
+  __shared__ int ired[16];
   const int b = blockIdx.x, len = draft_length(A, b), place = (int)A.accepted[b];
   VerifyBest a = A.best[(int64_t)b * A.n_race];
   for (int i = 1; i < A.n_race; ++i) best_merge(a, A.best[(int64_t)b * A.n_race + i]);
   VerifyDraw w{};
   w.place = place;
   if (!(a.lower > a.other)) w = draw_at<D>(A, b, place, len);
-  finish<D, 256>(A, b, w, a, red, ired);
+  finish<D, 1024>(A, b, w, a, red, ired);
 }
 
-static bool verify_whole(int B) { return B >= 64; }
-
+// A round is worth its launch (about 5 us) where it may save as much reading: the first takes two places, or as many as 64 MB of rows
+// are (10 us of reading), each further one twice as many.
+#define VERIFY_ROUND_BYTES (64 << 20)
+static int verify_first(const VerifyArgs& A, int dtype) {
+  const int64_t place = (int64_t)A.B * A.V * row_size(dtype) * (A.draft ? 2 : 1), n = (VERIFY_ROUND_BYTES + place - 1) / place;
+  return n < 2 ? 2 : n > A.N + 1 ? A.N + 1 : (int)n;
+}
+// Chunks: rows at most 2^15 elements, the draw up to there in one workgroup of 1024 (a join of its own costs as much as that takes:
+// 16 x 8 drafts x 50021 fp16 29 us in one workgroup, 25 in chunks; 32000 bf16 the same either way).
 static void verify_plan(VerifyArgs& A, int dtype) {
-  const int most = 1 << 15;
-  A.n_chunk = row_chunks(A.B * (A.draft ? 2 * A.N + 1 : A.N + 1), A.V, most, 1 << 13);
+  const int most = 1 << 15, first = verify_first(A, dtype);
+  A.n_chunk = row_chunks(A.B * first * (A.draft ? 2 : 1), A.V, most, 1 << 13);
   A.chunk = (A.V + A.n_chunk - 1) / A.n_chunk;
-  A.n_race = A.V <= 1 << 16 ? 1 : row_chunks(A.B, A.V, most, 1 << 13);
+  A.n_race = A.V <= most ? 1 : row_chunks(A.B, A.V, most, 1 << 13);
   A.race_chunk = (A.V + A.n_race - 1) / A.n_race;
 }
 
 extern "C" int64_t nast_verify_draft_workspace_bytes(int B, int N, int V, int dtype) {
-  if (B < 1 || N < 0 || N > VERIFY_MAX_DRAFTS || V < 1 || V > VERIFY_MAX_V || verify_whole(B)) return 0;
+  if (B < 1 || N < 0 || N > VERIFY_MAX_DRAFTS || V < 1 || V > VERIFY_MAX_V || !row_dtype_ok(dtype)) return 0;
   int64_t most = 0;
   for (int draft = 0; draft < 2; ++draft) {                   // (with and without draft logits)
     VerifyArgs A;
@@ -406,7 +418,7 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
                "nast_verify_draft: bad sizes B=%d N=%d V=%d", B, N, V);
   NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_verify_draft: temperature must be > 0 and finite");
   if (B == 0) return NAST_OK;
-  NAST_REQUIRE(target && E && out && accepted && (verify_whole(B) || workspace) && (N == 0 || (tokens && u)),
+  NAST_REQUIRE(target && E && out && accepted && workspace && (N == 0 || (tokens && u)),
                "nast_verify_draft: NULL pointer");
   NAST_REQUIRE(row_aligned(target, dtype) && row_aligned(draft, dtype), "nast_verify_draft: misaligned pointer");
   VerifyArgs A;
@@ -428,25 +440,26 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
   A.it = 1.0 / temp;
   A.c = exp_scale(temp);
   hipStream_t s = (hipStream_t)stream;
-  const int rows = B * (A.draft ? 2 * N + 1 : N + 1);
+  verify_plan(A, dtype);
+  NAST_REQUIRE((int64_t)B * (2 * N + 1) * A.n_chunk < (1 << 24) && (int64_t)B * A.n_race < (1 << 22), "nast_verify_draft: too many rows (%d)", B);
   nast_prof_before(2, s);
-  if (verify_whole(B)) {
-    NAST_ROW_DTYPE(dtype, hipLaunchKernelGGL((nast_verify_whole_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A));
-  } else {
-    verify_plan(A, dtype);
-    A.parts = (MaxSumD*)workspace;
-    A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
-    NAST_ROW_DTYPE(dtype, {
-      hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(rows * A.n_chunk), dim3(256), 0, s, A);
-      if (A.n_race == 1) {
-        hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
-      } else {
-        hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B * A.n_race), dim3(256), 0, s, A);
-        hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(256), 0, s, A);
-      }
-    });
-  }
-  nast_prof_after(2, s, (double)V * (row_size(dtype) * (double)rows + 4.0 * B));
+  A.parts = (MaxSumD*)workspace;
+  A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
+  NAST_ROW_DTYPE(dtype, {
+    for (int i0 = 0, n = verify_first(A, dtype); i0 <= N; i0 += n, n *= 2) {
+      if (n > N + 1 - i0) n = N + 1 - i0;
+      const int n_draft = !A.draft ? 0 : n < N - i0 ? n : N - i0;
+      hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(B * (n + n_draft) * A.n_chunk), dim3(256), 0, s, A, i0, n, n_draft);
+    }
+    if (A.n_race == 1) {
+      hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
+    } else {
+      hipLaunchKernelGGL((nast_verify_place_kernel<D>), dim3(B), dim3(1024), 0, s, A);
+      hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B * A.n_race), dim3(256), 0, s, A);
+      hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(1024), 0, s, A);
+    }
+  });
+  nast_prof_after(2, s, (double)V * B * (row_size(dtype) * (A.draft ? 2.0 * N + 1 : N + 1.0) + 4.0));
   NAST_CHECK_LAUNCH("nast_verify_draft");
   return NAST_OK;
 }
