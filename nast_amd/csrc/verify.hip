@@ -125,8 +125,9 @@ __device__ __forceinline__ VerifyDraw draw_of(const VerifyArgs& A, int b, int pl
   return w;
 }
 
-// Argmax of w / E over [lo, hi) in fp32 with error bounds, by the whole workgroup.  An element is looked at closer only where its upper
-// bound exceeds the best lower bound that its wavefront has seen.
+// Argmax of w / E over [lo, hi) in fp32 with error bounds, by the whole workgroup.  Most elements are told apart by one logarithm:
+// log2(p / E), not less than the logarithm of their score, against that of the best lower bound their wavefront has seen (less 0.01, a
+// thousand times what the two are off by).  Only what passes is looked at closer.
 template <class D, int NT>
 __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int lo, int hi, VerifyBest* lds) {
   VerifyBest a{0.f, 0.f, 0.f, 0.f, 0x7fffffff};
@@ -137,9 +138,11 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     const float pm = (float)w.p.m, qm = (float)w.q.m, ps = -(float)log2(w.p.s), qs = w.minus_q ? -(float)log2(w.q.s) : 0.f;
     const float slope = -VERIFY_REL_EXP * A.c;
     float seen = 0.f;
+    float seen_log = -INFINITY;
     auto look = [&](float zp, float zq, float en, int e) {
-      const float tp = zp - pm, tq = zq - qm;
-      const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(tp, A.c, ps));
+      const float tp = zp - pm, log_p = __builtin_fmaf(tp, A.c, ps);
+      if (log_p - __builtin_amdgcn_logf(en) < seen_log) return;   // (a draw of 0 or NaN passes)
+      const float tq = zq - qm, pv = __builtin_amdgcn_exp2f(log_p);
       const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(tq, A.c, qs)) : 0.f;
       const float d = pv - qv, inv = __builtin_amdgcn_rcpf(en);
       const float err = 1e-37f + (pv * __builtin_fmaf(tp, slope, VERIFY_REL) + (q ? qv * __builtin_fmaf(tq, slope, VERIFY_REL) : 0.f));
@@ -153,7 +156,6 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     for (int b0 = 0; b0 < rs.n; b0 += NT * U) {
       RowVec<D> pv[U], qv[U];
       RowVec<RowF32> ev[U][W];
-      seen = wave_max(fmaxf(seen, a.lower));                    // (every lane takes part)
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int at = rs.elem(min(b0 + NT * i + (int)threadIdx.x, rs.n - 1));
@@ -164,6 +166,8 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
+        seen = wave_max(fmaxf(seen, a.lower));                  // (every lane takes part)
+        seen_log = __builtin_amdgcn_logf(seen) - 0.01f;
         const int s = b0 + NT * i + (int)threadIdx.x;
         if (s < rs.n)
 #pragma unroll
@@ -249,8 +253,8 @@ __device__ void finish(const VerifyArgs& A, int b, const VerifyDraw& w, const Ve
 
 // ---------------------------------------------------------------------------------------------
 // Rows are read in rounds of places, each a launch over (sequence, row, chunk); a round leaves out the sequences that a clear refusal of
-// an earlier one has ended, whose further rows nothing needs.  Then place and draw: by one workgroup a sequence, or the draw in chunks,
-// with a launch before it that finds the place and one behind it that joins them.
+// an earlier one has ended, whose further rows nothing needs.  Then place and draw: by one workgroup a sequence, or in chunks, each
+// workgroup finding the place for itself, and a launch that joins them.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
   const MaxSumD* q = A.parts + (int64_t)row * A.n_chunk;
@@ -345,24 +349,18 @@ __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
   __shared__ int ired[NT / 64];
   __shared__ VerifyBest lds[NT / 64];
   const int b = blockIdx.x / A.n_race, lo = (int)(blockIdx.x % A.n_race) * A.race_chunk, hi = min(A.V, lo + A.race_chunk);
-  const int len = draft_length(A, b), place = A.n_race == 1 ? places<D, NT>(A, b, len, red) : (int)A.accepted[b];
+  const int len = draft_length(A, b), place = places<D, NT>(A, b, len, red);
   const VerifyDraw w = draw_at<D>(A, b, place, len);
   const VerifyBest a = race<D, NT>(A, b, w, lo, hi, lds);
   if (A.n_race == 1) {
     finish<D, NT>(A, b, w, a, red, ired);
   } else if (threadIdx.x == 0) {
     A.best[blockIdx.x] = a;
+    if (lo == 0) A.accepted[b] = place;
   }
 }
 
-// (1024 threads in these two for the sums in double that they may have to make)
-template <class D>
-__global__ __launch_bounds__(1024) void nast_verify_place_kernel(VerifyArgs A) {
-  __shared__ double red[16];
-  const int b = blockIdx.x, place = places<D, 1024>(A, b, draft_length(A, b), red);
-  if (threadIdx.x == 0) A.accepted[b] = place;
-}
-
+// (1024 threads for the draw in double that it may have to make)
 template <class D>
 __global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
   __shared__ double red[16];
@@ -376,17 +374,19 @@ __global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
   finish<D, 1024>(A, b, w, a, red, ired);
 }
 
-// A round is worth its launch (about 5 us) where it may save as much reading: the first takes two places, or as many as 64 MB of rows
-// are (10 us of reading), each further one twice as many.
+// A round is worth its launch (about 5 us) where it may save as much reading, 64 MB of rows (10 us).  So many places at least has
+// each, the first two or more, the next ones twice as many as the one before; where less is left than that it is taken along.
 #define VERIFY_ROUND_BYTES (64 << 20)
-static int verify_first(const VerifyArgs& A, int dtype) {
-  const int64_t place = (int64_t)A.B * A.V * row_size(dtype) * (A.draft ? 2 : 1), n = (VERIFY_ROUND_BYTES + place - 1) / place;
-  return n < 2 ? 2 : n > A.N + 1 ? A.N + 1 : (int)n;
+static int verify_round(const VerifyArgs& A, int dtype, int i0, int last) {
+  const int64_t place = (int64_t)A.B * A.V * row_size(dtype) * (A.draft ? 2 : 1), least = (VERIFY_ROUND_BYTES + place - 1) / place;
+  const int left = A.N + 1 - i0;
+  const int64_t n = least > 2 * last ? least : 2 * last;
+  return n + least >= left ? left : (int)n;
 }
 // Chunks: rows at most 2^15 elements, the draw up to there in one workgroup of 1024 (a join of its own costs as much as that takes:
 // 16 x 8 drafts x 50021 fp16 29 us in one workgroup, 25 in chunks; 32000 bf16 the same either way).
 static void verify_plan(VerifyArgs& A, int dtype) {
-  const int most = 1 << 15, first = verify_first(A, dtype);
+  const int most = 1 << 15, first = verify_round(A, dtype, 0, 1);
   A.n_chunk = row_chunks(A.B * first * (A.draft ? 2 : 1), A.V, most, 1 << 13);
   A.chunk = (A.V + A.n_chunk - 1) / A.n_chunk;
   A.n_race = A.V <= most ? 1 : row_chunks(A.B, A.V, most, 1 << 13);
@@ -446,15 +446,14 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
   A.parts = (MaxSumD*)workspace;
   A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
   NAST_ROW_DTYPE(dtype, {
-    for (int i0 = 0, n = verify_first(A, dtype); i0 <= N; i0 += n, n *= 2) {
-      if (n > N + 1 - i0) n = N + 1 - i0;
+    for (int i0 = 0, n = 1; i0 <= N; i0 += n) {
+      n = verify_round(A, dtype, i0, n);
       const int n_draft = !A.draft ? 0 : n < N - i0 ? n : N - i0;
       hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(B * (n + n_draft) * A.n_chunk), dim3(256), 0, s, A, i0, n, n_draft);
     }
     if (A.n_race == 1) {
       hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
     } else {
-      hipLaunchKernelGGL((nast_verify_place_kernel<D>), dim3(B), dim3(1024), 0, s, A);
       hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B * A.n_race), dim3(256), 0, s, A);
       hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(1024), 0, s, A);
     }

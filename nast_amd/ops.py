@@ -6,6 +6,7 @@ There is no CPU / eager fallback: a non-CUDA tensor raises.
 """
 import collections
 import ctypes as C
+import functools
 import math
 import os
 
@@ -1137,16 +1138,15 @@ of all its logits at `temperature` (fp32; None where only the list is known)."""
 
 def _on_device(first, *rest):
     """The raw stream to launch on.  All tensors have to live on the current device: kernels are launched there."""
-    for t in (first,) + rest:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise _lib.NastHipError("nast_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
-        if t.device != first.device:
-            raise _lib.NastHipError(f"tensors on two devices: {first.device} and {t.device}")
-    if first.device.index != torch.cuda.current_device():
-        raise _lib.NastHipError(f"tensors on {first.device}, the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(first.device.index)
+    dev = first.device
+    if dev.type != "cuda":
+        raise _lib.NastHipError("nast_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback")
+    for t in rest:
+        if t is not None and t.device != dev:
+            raise _lib.NastHipError(f"tensors on two devices: {dev} and {t.device}")
+    if dev.index != torch._C._cuda_getDevice():
+        raise _lib.NastHipError(f"tensors on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream if _raw_stream is None else _raw_stream(dev.index)
 
 
 def _row_dtype(t):
@@ -1169,8 +1169,14 @@ def _vocab_rows(t):
     return t, r, rows
 
 
-def _workspace(nbytes, like):
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    return getattr(load(), name)(*sizes)
+
+
+def _workspace(like, name, *sizes):
+    n = _workspace_bytes(name, *sizes)
+    return torch.empty(n, dtype=torch.uint8, device=like.device) if n else None
 
 
 def _positive(temperature):
@@ -1184,7 +1190,8 @@ def top_logits(logits, k, temperature=1.0):
     """The k largest logits of every row of logits [..., V] and the row's log-sum-exp at `temperature`: TopLogits with values
     [..., k] (the logits' type, largest first, ties to the lower id, NaN above everything), index [..., k] int64, lse [...] fp32.
     1 <= k <= min(256, V).  No gradient flows: this is the teacher's side."""
-    logits = logits.detach()
+    if logits.requires_grad:
+        logits = logits.detach()
     stream, dtype, temperature, k = _on_device(logits), _row_dtype(logits), _positive(temperature), int(k)
     x, r, rows = _vocab_rows(logits)
     V = x.shape[-1]
@@ -1194,15 +1201,15 @@ def top_logits(logits, k, temperature=1.0):
     values = torch.empty(*lead, k, device=x.device, dtype=x.dtype)
     index = torch.empty(*lead, k, device=x.device, dtype=torch.int64)
     lse = torch.empty(lead, device=x.device, dtype=F32)
-    ws = _workspace(load().nast_top_logits_workspace_bytes(rows, V, k, dtype), x)
+    ws = _workspace(x, "nast_top_logits_workspace_bytes", rows, V, k, dtype)
     call("nast_top_logits", _p(x), dtype, r, _p(values), _p(index), _p(lse), rows, V, k, temperature, _p(ws), stream)
     return TopLogits(values, index, lse, temperature)
 
 
 def _teacher_list(lead, top, temperature, tail):
     """(values, index, lse or None) of a TopLogits, checked against the rows it belongs to."""
-    values, index, lse = top.values.detach(), top.index, top.lse
-    if values.dim() == 0 or tuple(values.shape[:-1]) != tuple(lead) or index.shape != values.shape:
+    values, index, lse = top[:3]
+    if values.dim() == 0 or values.shape[:-1] != lead or index.shape != values.shape:
         raise _lib.NastHipError(f"teacher's list: values {tuple(values.shape)} and index {tuple(index.shape)} for rows {tuple(lead)}")
     if not 1 <= values.shape[-1] <= 256:
         raise _lib.NastHipError(f"a teacher's list has 1 to 256 slots, not {values.shape[-1]}")
@@ -1211,31 +1218,31 @@ def _teacher_list(lead, top, temperature, tail):
     _row_dtype(values)
     if not tail:
         return _c(values), _c(index), None
-    if lse is None or lse.dtype != F32 or tuple(lse.shape) != tuple(lead):
+    if lse is None or lse.dtype != F32 or lse.shape != lead:
         raise _lib.NastHipError("tail=True needs the teacher's log-sum-exp, fp32, one per row")
     if top.temperature != temperature:
         raise _lib.NastHipError(f"the teacher's log-sum-exp was taken at temperature {top.temperature}, not {temperature}")
-    return _c(values), _c(index), _c(lse.detach())
+    return _c(values), _c(index), _c(lse)
 
 
-def _distill_fwd(x, r, rows, dtype, teacher, temperature, stream):
-    """-> loss [rows] fp32, stats [rows, 6] double"""
+def _distill_fwd(x, r, rows, lead, dtype, teacher, temperature, stream):
+    """-> loss [lead] fp32, stats [rows, 6] double"""
     values, index, lse = teacher
-    V, K = x.shape[-1], values.shape[-1]
-    loss = torch.empty(rows, device=x.device, dtype=F32)
-    stats = torch.empty(rows, 6, device=x.device, dtype=torch.float64)
-    ws = _workspace(load().nast_top_distill_workspace_bytes(rows, V, dtype), x)
-    call("nast_top_distill_fwd", _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), K, _p(lse), _p(loss), _p(stats), rows, V,
-         temperature, _p(ws), stream)
+    V, dev = x.shape[-1], x.device
+    loss = torch.empty(lead, device=dev, dtype=F32)
+    stats = torch.empty(rows, 6, device=dev, dtype=torch.float64)
+    ws = _workspace(x, "nast_top_distill_workspace_bytes", rows, V, dtype)
+    call("nast_top_distill_fwd", _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), values.shape[-1], _p(lse), _p(loss),
+         _p(stats), rows, V, temperature, _p(ws), stream)
     return loss, stats
 
 
 def _distill_bwd(g, x, r, rows, dtype, values, index, stats, temperature, stream):
     """-> d loss / d logits, contiguous, in the logits' type"""
-    V, K = x.shape[-1], values.shape[-1]
-    gx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    call("nast_top_distill_bwd", _p(g), _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), K, _p(stats), _p(gx), Rows(V, 0, 0),
-         rows, V, temperature, stream)
+    V = x.shape[-1]
+    gx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    call("nast_top_distill_bwd", _p(g), _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), values.shape[-1], _p(stats), _p(gx),
+         Rows(V, 0, 0), rows, V, temperature, stream)
     return gx
 
 
@@ -1244,21 +1251,22 @@ class TopDistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, top, temperature, tail):
-        teacher = _teacher_list(logits.shape[:-1], top, temperature, tail)
+        lead = logits.shape[:-1]
+        teacher = _teacher_list(lead, top, temperature, tail)
         stream, dtype = _on_device(logits, *teacher), _row_dtype(logits)
         x, r, rows = _vocab_rows(logits)
-        loss, stats = _distill_fwd(x, r, rows, dtype, teacher, temperature, stream)
-        ctx.save_for_backward(logits, teacher[0], teacher[1], stats)
-        ctx.temperature = temperature
-        return loss.view(logits.shape[:-1])
+        loss, stats = _distill_fwd(x, r, rows, lead, dtype, teacher, temperature, stream)
+        ctx.save_for_backward(x, teacher[0], teacher[1], stats)
+        ctx.call, ctx.shape = (r, rows, dtype, temperature), logits.shape
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        logits, values, index, stats = ctx.saved_tensors
-        x, r, rows = _vocab_rows(logits)
-        gx = _distill_bwd(_c(g).view(-1), x, r, rows, _ROW_DTYPES[x.dtype], values, index, stats, ctx.temperature, _on_device(logits, g))
-        return gx.view(logits.shape), None, None, None
+        x, values, index, stats = ctx.saved_tensors
+        r, rows, dtype, temperature = ctx.call
+        gx = _distill_bwd(_c(g), x, r, rows, dtype, values, index, stats, temperature, _on_device(x, g))
+        return gx.view(ctx.shape), None, None, None
 
 
 def top_distill(logits, top, temperature=1.0, tail=False):
@@ -1286,17 +1294,17 @@ class GeneratorDistillFn(torch.autograd.Function):
         y = torch.empty(x2.shape[0], V, device=x.device, dtype=F32)
         if x2.shape[0]:
             gemm([d_fwd(x2, W, y, bias=b)])
-        loss, stats = _distill_fwd(y, Rows(V, 0, 0), y.shape[0], 0, teacher, temperature, stream)
+        loss, stats = _distill_fwd(y, Rows(V, 0, 0), y.shape[0], x.shape[:-1], 0, teacher, temperature, stream)
         ctx.save_for_backward(x2, W, y, teacher[0], teacher[1], stats)
         ctx.params = live(W, b)
         ctx.temperature, ctx.xshape = temperature, x.shape
-        return loss.view(x.shape[:-1])
+        return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         x2, W, y, values, index, stats = ctx.saved_tensors
-        gl = _distill_bwd(_c(g).view(-1), y, Rows(W.shape[0], 0, 0), y.shape[0], 0, values, index, stats, ctx.temperature, _on_device(y, g))
+        gl = _distill_bwd(_c(g), y, Rows(W.shape[0], 0, 0), y.shape[0], 0, values, index, stats, ctx.temperature, _on_device(y, g))
         (dW, db), (rW, rb) = grad_buffers(list(ctx.params))
         dx = torch.empty_like(x2)
         if x2.shape[0]:
@@ -1322,20 +1330,19 @@ def verify_draft(target, tokens, u, E, draft=None, lengths=None, temperature=1.0
     With p_i, q_i the softmax of the rows over `temperature`, draft i stands while u_i q_i(d_i) < p_i(d_i) (and q_i(d_i) > 0).  out
     holds the drafts that stand, then argmax (p_i - q_i)+ / E at the first that falls (p_N / E if none does), then -1.  A target row
     without a distribution (a NaN, a +inf, nothing but -inf) lets nothing stand and gives -1."""
-    target, draft = target.detach(), None if draft is None else draft.detach()
     stream, dtype, temperature = _on_device(target, tokens, u, E, draft, lengths), _row_dtype(target), _positive(temperature)
     if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
         raise _lib.NastHipError(f"target logits [B, N + 1, V] expected, got {tuple(target.shape)}")
     B, N, V = target.shape[0], target.shape[1] - 1, target.shape[2]
     for name, t, shape, kind in (("tokens", tokens, (B, N), torch.int64), ("u", u, (B, N), F32), ("E", E, (B, V), F32),
                                  ("draft", draft, (B, N, V), target.dtype), ("lengths", lengths, (B,), torch.int64)):
-        if t is not None and (tuple(t.shape) != shape or t.dtype != kind):
+        if t is not None and (t.shape != shape or t.dtype != kind):
             raise _lib.NastHipError(f"{name}: {shape} {kind} expected, got {tuple(t.shape)} {t.dtype}")
     target, draft = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (target, draft))
     tokens, u, E, lengths = (None if t is None else _c(t) for t in (tokens, u, E, lengths))
     out = torch.empty(B, N + 1, device=target.device, dtype=torch.int64)
     accepted = torch.empty(B, device=target.device, dtype=torch.int64)
-    ws = _workspace(load().nast_verify_draft_workspace_bytes(B, N, V, dtype), target)
+    ws = _workspace(target, "nast_verify_draft_workspace_bytes", B, N, V, dtype)
     call("nast_verify_draft", _p(target), target.stride(0), target.stride(1), _p(draft), *((0, 0) if draft is None else draft.stride()[:2]),
          dtype, _p(tokens), _p(u), _p(E), _p(lengths), _p(out), _p(accepted), B, N, V, temperature, _p(ws), stream)
     return out, accepted
