@@ -136,7 +136,7 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     const typename D::store* q = w.minus_q ? draft_row<D>(A, b, w.place) : nullptr;
     const float* E = A.E + (int64_t)b * A.V;
     const float pm = (float)w.p.m, qm = (float)w.q.m, ps = -(float)log2(w.p.s), qs = w.minus_q ? -(float)log2(w.q.s) : 0.f;
-    const float slope = -VERIFY_REL_EXP * A.c;
+    const float slope = -VERIFY_REL_EXP * A.c, far = -200.f / A.c;
     float seen = 0.f;
     float seen_log = -INFINITY;
     auto look = [&](float zp, float zq, float en, int e) {
@@ -145,7 +145,9 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
       const float tq = zq - qm, pv = __builtin_amdgcn_exp2f(log_p);
       const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(tq, A.c, qs)) : 0.f;
       const float d = pv - qv, inv = __builtin_amdgcn_rcpf(en);
-      const float err = 1e-37f + (pv * __builtin_fmaf(tp, slope, VERIFY_REL) + (q ? qv * __builtin_fmaf(tq, slope, VERIFY_REL) : 0.f));
+      // (below 2^-150 the bound is the absolute one; an exponent of -inf would make it 0 * inf)
+      const float ep = pv * __builtin_fmaf(fmaxf(tp, far), slope, VERIFY_REL), eq = q ? qv * __builtin_fmaf(fmaxf(tq, far), slope, VERIFY_REL) : 0.f;
+      const float err = 1e-37f + (ep + eq);
       const float upper = (d + err) * inv;
       if (upper > seen && e != w.one) best_merge(a, {d * inv, (d - err) * inv, upper, 0.f, e});
     };

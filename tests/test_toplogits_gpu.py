@@ -348,6 +348,19 @@ def test_verify_draft(ops, dtype, B, N, V):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 5003, 40001])
+def test_verify_draft_filtered_rows(ops, dtype, V):
+    """improbable words cut off (-inf) on both sides, most of what is drawn from has no probability in the draft"""
+    for seed in range(6):
+        target, tokens, u, E, draft = drafts(16, 3, V, dtype, seed + V, noise=0.8)
+        target = target.masked_fill(target < target.amax(-1, keepdim=True) - 7, -INF)
+        draft = draft.masked_fill(draft < draft.amax(-1, keepdim=True) - 6, -INF)
+        lengths = (torch.arange(16) % 4).cuda()
+        check_verify(ops, target, draft.argmax(-1), u, E, draft, lengths, 0.8)
+        check_verify(ops, target, tokens, u, E, None, lengths, 0.8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_verify_draft_unusual_rows(ops, dtype):
     B, N, V = 12, 3, 501
     target, tokens, u, E, draft = drafts(B, N, V, dtype, 11, noise=0.3)
