@@ -60,6 +60,11 @@ template <class D>
 __device__ __forceinline__ void vec_store(typename D::store* p, const RowVec<D>& v) {
   *reinterpret_cast<uint4*>(p) = make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
 }
+typedef uint32_t raw16 __attribute__((ext_vector_type(4)));
+template <class D>
+__device__ __forceinline__ void vec_store_around(typename D::store* p, const RowVec<D>& v) {   // not kept in the last-level cache
+  __builtin_nontemporal_store(raw16{v.w[0], v.w[1], v.w[2], v.w[3]}, reinterpret_cast<raw16*>(p));
+}
 // 16 bytes from any element: global_load_dwordx4 takes any alignment on this target
 typedef uint32_t raw16_any __attribute__((ext_vector_type(4), aligned(2)));
 template <class D>

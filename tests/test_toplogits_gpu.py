@@ -108,6 +108,18 @@ def test_top_logits_strides_and_alignment(ops, dtype):
     assert ops.top_logits(base.view(4, 6, 1003)[:, :0], 4).lse.shape == (4, 0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_logits_largest(ops, dtype):
+    """the longest rows and lists: as many entries to join as there can be; ties, a NaN and -inf across the chunks"""
+    V, k = 1 << 20, 256
+    x = rows(5, V, dtype, 1)
+    x[1] = 0.5
+    x[2] = x[2].sort(descending=True).values
+    x[3, ::4097] = float("nan")
+    x[4, 100:-100] = -INF
+    check_top(ops, x, k)
+
+
 def test_top_logits_far_offsets(ops):
     """rows that lie beyond 2^31 elements of their tensor"""
     R, V = 20000, 120000
@@ -259,6 +271,80 @@ def test_top_distill_strides(ops, dtype):
     empty.sum().backward()
 
 
+def test_top_distill_large_gradient(ops):
+    """a gradient larger than the last-level cache, rows picked from it"""
+    R, V, K = 600, 131075, 9
+    x = rows(R, V, torch.float32, 5).requires_grad_()
+    index = torch.randint(0, V, (R, K), generator=torch.Generator().manual_seed(1)).cuda()
+    index[:, 3] = index[:, 4]
+    values = x.detach().gather(1, index) + 3.0
+    lse = torch.logsumexp(x.detach(), 1) + 2.5
+    g = torch.rand(R, device="cuda")
+    for tail in (False, True):
+        loss = ops.top_distill(x, ops.TopLogits(values, index, lse, 1.0), 1.0, tail=tail)
+        (grad,) = torch.autograd.grad(loss, x, g)
+        pick = torch.tensor([0, 1, 299, R - 1], device="cuda")
+        wl, wg, ws = oracle.distill(x.detach()[pick], values[pick], index[pick], lse[pick], 1.0, tail, g[pick])
+        assert ((loss[pick].detach().cpu().double() - wl).abs() <= EPS + wl.abs() * 2.0 ** -24).all()
+        check_grad(grad[pick], wg, ws)
+
+
+def test_top_distill_autograd(ops):
+    """the graph kept and walked twice, a broadcast leaf, a leaf changed in between, a second derivative refused"""
+    x = rows(1, 77, torch.float32, 4).requires_grad_()
+    v, i, lse = teacher_of(x.detach().expand(6, 77).contiguous(), 5, 1.0, 2)
+    top = ops.TopLogits(v, i, lse, 1.0)
+    loss = ops.top_distill(x.expand(6, 77), top, 1.0, tail=True).sum()
+    (a,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (b,) = torch.autograd.grad(loss, x)
+    want = oracle.distill(x.detach().expand(6, 77), v, i, lse, 1.0, True, torch.ones(6))
+    assert torch.equal(a, b)
+    check_grad(a, want[1].sum(0, keepdim=True), want[2].sum(0, keepdim=True) + 6 * want[1].abs().sum(0, keepdim=True) * 2.0 ** -24 / EPS)
+    leaf = rows(6, 77, torch.float32, 4).requires_grad_()
+    loss = ops.top_distill(leaf, top).sum()
+    with torch.no_grad():
+        leaf.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+    w = torch.ones(6, device="cuda", requires_grad=True)
+    (first,) = torch.autograd.grad((ops.top_distill(leaf, top) * w).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        first.sum().backward()
+
+
+def test_refusals(ops):
+    from nast_amd._lib import NastHipError
+    x = rows(4, 50, torch.float32, 1)
+    for bad, match in ((x.double(), "fp32, bf16 or fp16"), (x.long(), "fp32, bf16 or fp16"), (x.t(), "contiguous"), (x[:, :0], "vocabulary axis"),
+                       (torch.tensor(1.0, device="cuda"), "vocabulary axis")):
+        with pytest.raises(NastHipError, match=match):
+            ops.top_logits(bad, 1)
+        with pytest.raises(NastHipError, match=match):
+            lead = bad.shape[:-1] if bad.dim() else ()
+            ops.top_distill(bad, ops.TopLogits(torch.zeros(*lead, 1, device="cuda"), torch.zeros(*lead, 1, dtype=torch.int64, device="cuda"), None, 1.0))
+    for k in (0, -1, 51, 257):
+        with pytest.raises(NastHipError, match="k="):
+            ops.top_logits(x, k)
+    with pytest.raises(NastHipError, match="temperature"):
+        ops.top_logits(x, 1, 0.0)
+    with pytest.raises(NastHipError, match="bad sizes"):
+        ops.top_logits(torch.zeros(1, (1 << 20) + 1, device="cuda"), 1)
+    top = ops.top_logits(x, 3)
+    with pytest.raises(NastHipError, match="two devices"):
+        ops.top_distill(x, top._replace(index=top.index.cpu()))
+    with pytest.raises(NastHipError, match="temperature"):
+        ops.top_distill(x, top, 2.0, tail=True)
+    target, tokens, u, E, draft = drafts(2, 3, 50, torch.float32, 1)
+    good = dict(target=target, tokens=tokens, u=u, E=E, draft=draft, lengths=None, temperature=1.0)
+    for name, bad, match in (("target", target[0], "B, N"), ("target", target.double(), "fp32, bf16"), ("tokens", tokens.int(), "tokens"),
+                             ("tokens", tokens[:, :2], "tokens"), ("u", u.double(), "u:"), ("u", u[:1], "u:"), ("E", E[:, :49], "E:"),
+                             ("E", E.half(), "E:"), ("draft", draft.half(), "draft"), ("draft", target, "draft"), ("lengths", torch.ones(2, device="cuda"), "lengths"),
+                             ("lengths", torch.ones(3, dtype=torch.int64, device="cuda"), "lengths"), ("temperature", 0.0, "temperature"),
+                             ("E", E.cpu(), "two devices"), ("draft", draft.cpu(), "two devices")):
+        with pytest.raises(NastHipError, match=match):
+            ops.verify_draft(**{**good, name: bad})
+
+
 def test_top_distill_differences(ops):
     """the gradient against central differences of the loss: a loss within 2e-7 divided by 2h = 0.05, plus h^2 / 6 of a third
     derivative below 0.2"""
@@ -384,12 +470,12 @@ def test_verify_draft_unusual_rows(ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_verify_draft_borders(ops, dtype):
+@pytest.mark.parametrize("V", [64, 40000])
+def test_verify_draft_borders(ops, dtype, V):
     """comparisons that fp32 cannot decide: a ratio next to u, equal scores, p and q nearly the same, a residual of nothing"""
-    V = 64
-    target = torch.zeros(4, 2, V, dtype=dtype, device="cuda")            # p = 1/64 everywhere
+    target = torch.zeros(4, 2, V, dtype=dtype, device="cuda")            # p = 1/V everywhere
     draft = torch.zeros(4, 1, V, dtype=dtype, device="cuda")
-    draft[:, :, V // 2:] = -INF                                          # q = 1/32 on the lower half: ratio 1/2
+    draft[:, :, V // 2:] = -INF                                          # q = 2/V on the lower half: ratio 1/2
     tokens = torch.zeros(4, 1, dtype=torch.int64, device="cuda")
     half = torch.tensor(0.5)
     u = torch.stack([torch.nextafter(half, half * 0), torch.nextafter(half, half * 2), half * 0, half * 2]).view(4, 1).cuda()
@@ -440,6 +526,16 @@ def test_verify_draft_distribution(ops):
         with U.inject_noise([torch.zeros(4, 1, device="cuda"), torch.ones(4, V, device="cuda")]):
             again, _ = U.verify_draft(target.expand(4, 2, V), tokens[:4], draft.expand(4, 1, V))
         assert torch.equal(again[:, :1], tokens[:4]) and (again[:, 1] == p[1].argmax()).all()
+
+
+@pytest.mark.parametrize("with_q", [True, False])
+def test_verify_draft_in_rounds(ops, with_q):
+    """a batch whose rows are read in more than one round, sequences that end in each of them"""
+    target, tokens, u, E, draft = drafts(64, 8, 50021, torch.float32, 21, noise=0.1, scale=3.0)
+    lengths = (torch.arange(64) % 9).cuda()
+    lengths[::2] = 8
+    _, accepted = check_verify(ops, target, tokens if with_q else target[:, :8].argmax(-1), u if with_q else u * 0.3, E, draft if with_q else None, lengths)
+    assert len(set(accepted.tolist())) > 4
 
 
 # ------------------------------------------------------------------------------------------------

@@ -12,10 +12,9 @@ def top(logits, k, temp):
     """-> index [R, k], lse [R]"""
     index, lse = [], []
     for x in _rows(logits):
-        order = sorted(range(x.numel()), key=lambda v: (0, 0, v) if math.isnan(x[v]) else (1, -x[v].item(), v))
-        index.append(order[:k])
+        index.append(torch.sort(x, descending=True, stable=True).indices[:k])     # NaN first, equal ones in their order
         lse.append(torch.logsumexp(x / temp, 0))
-    return torch.tensor(index, dtype=torch.int64).reshape(-1, k), torch.stack(lse) if lse else torch.empty(0, dtype=torch.float64)
+    return torch.stack(index), torch.stack(lse)
 
 
 def distill(logits, values, index, lse, temp, tail, g):
