@@ -29,6 +29,7 @@ struct VerifyArgs {
   int race_chunk, n_race;         // of the draw
   MaxSumD* parts;                 // [B * (2 N + 1)][n_chunk]: target rows first, then draft rows
   struct VerifyBest* best;        // [B][n_race]
+  int* ended;                     // [B]
 };
 
 // the running argmax of the draw: score, bounds of the exact score, the largest upper bound of any other, where
@@ -282,29 +283,29 @@ __device__ __forceinline__ VerifyPair drafted_at(const VerifyArgs& A, int b, int
   return drafted<D>(A, b, i, row_pair(A, b * (A.N + 1) + i), A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + i) : MaxSumD{0, 1});
 }
 
+// Between two rounds, one wavefront a sequence: whether a draft before place i0 is clearly refused.
+template <class D>
+__global__ __launch_bounds__(64) void nast_verify_ended_kernel(VerifyArgs A, int i0) {
+  const int b = blockIdx.x, len = draft_length(A, b);
+  bool ended = false;
+  for (int i = threadIdx.x; i < i0 && i < len; i += 64) {
+    const VerifyPair r = drafted_at<D>(A, b, i);
+    const float u = A.u[(int64_t)b * A.N + i];
+    ended = ended || (!stands(r, u) && !too_close(r, u));
+  }
+  const uint64_t any = __ballot(ended);
+  if (threadIdx.x == 0) A.ended[b] = any != 0 || len < i0;
+}
+
 template <class D>
 __global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A, int i0, int n_target, int n_draft) {
   __shared__ double red[8];
-  __shared__ int over;
   const int k = blockIdx.x / A.n_chunk, ch = blockIdx.x % A.n_chunk, lo = ch * A.chunk, hi = min(A.V, lo + A.chunk);
   const int b = k / (n_target + n_draft), j = k % (n_target + n_draft), len = draft_length(A, b);
   const bool is_target = j < n_target;
   const int i = i0 + (is_target ? j : j - n_target);
   if (is_target ? i > len : i >= len) return;
-  if (i0 > 0) {                                                // i0 <= len here
-    if (threadIdx.x < 64) {
-      bool ended = false;
-      for (int l = threadIdx.x; l < i0; l += 64) {
-        const VerifyPair r = drafted_at<D>(A, b, l);
-        const float u = A.u[(int64_t)b * A.N + l];
-        ended = ended || (!stands(r, u) && !too_close(r, u));
-      }
-      const uint64_t any = __ballot(ended);
-      if (threadIdx.x == 0) over = any != 0;
-    }
-    __syncthreads();
-    if (over) return;
-  }
+  if (i0 > 0 && A.ended[b]) return;
   const MaxSum a = span_max_sum<D, 256>(is_target ? target_row<D>(A, b, i) : draft_row<D>(A, b, i), lo, hi, A.c);
   const MaxSumD t = block_max_sum<256>(a, A.c, red);
   if (threadIdx.x == 0) A.parts[(int64_t)(is_target ? b * (A.N + 1) + i : A.B * (A.N + 1) + b * A.N + i) * A.n_chunk + ch] = t;
@@ -376,9 +377,11 @@ __global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
   finish<D, 1024>(A, b, w, a, red, ired);
 }
 
-// A round is worth its launch (about 5 us) where it may save as much reading, 64 MB of rows (10 us).  So many places at least has
-// each, the first two or more, the next ones twice as many as the one before; where less is left than that it is taken along.
-#define VERIFY_ROUND_BYTES (64 << 20)
+// A further round costs two launches (10 us) and saves the rows of the sequences that have ended, half of them perhaps: it has to have
+// 128 MB of rows (20 us).  So many places at least has each, the first two or more, the next ones twice as many as the one before; where
+// less is left than that it is taken along.  256 x 8 drafts x 131072 bf16 in rounds of 2, 4, 3 places 199 us, at once 249; 512 x 32 x 9600
+// fp32 129 and 247; 64 x 8 x 131072 76 at once, 82 in the same three rounds.
+#define VERIFY_ROUND_BYTES (128 << 20)
 static int verify_round(const VerifyArgs& A, int dtype, int i0, int last) {
   const int64_t place = (int64_t)A.B * A.V * row_size(dtype) * (A.draft ? 2 : 1), least = (VERIFY_ROUND_BYTES + place - 1) / place;
   const int left = A.N + 1 - i0;
@@ -405,7 +408,8 @@ extern "C" int64_t nast_verify_draft_workspace_bytes(int B, int N, int V, int dt
     A.V = V;
     A.draft = draft ? &A : nullptr;
     verify_plan(A, dtype);
-    const int64_t n = (int64_t)B * (2 * N + 1) * A.n_chunk * (int64_t)sizeof(MaxSumD) + (int64_t)B * A.n_race * (int64_t)sizeof(VerifyBest);
+    const int64_t n = (int64_t)B * (2 * N + 1) * A.n_chunk * (int64_t)sizeof(MaxSumD) + (int64_t)B * A.n_race * (int64_t)sizeof(VerifyBest) +
+                      (int64_t)B * (int64_t)sizeof(int);
     most = n > most ? n : most;
   }
   return most;
@@ -447,9 +451,11 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
   nast_prof_before(2, s);
   A.parts = (MaxSumD*)workspace;
   A.best = (VerifyBest*)(A.parts + (int64_t)B * (2 * N + 1) * A.n_chunk);
+  A.ended = (int*)(A.best + (int64_t)B * A.n_race);
   NAST_ROW_DTYPE(dtype, {
     for (int i0 = 0, n = 1; i0 <= N; i0 += n) {
       n = verify_round(A, dtype, i0, n);
+      if (i0) hipLaunchKernelGGL((nast_verify_ended_kernel<D>), dim3(B), dim3(64), 0, s, A, i0);
       const int n_draft = !A.draft ? 0 : n < N - i0 ? n : N - i0;
       hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(B * (n + n_draft) * A.n_chunk), dim3(256), 0, s, A, i0, n, n_draft);
     }

@@ -530,12 +530,20 @@ def test_verify_draft_distribution(ops):
 
 @pytest.mark.parametrize("with_q", [True, False])
 def test_verify_draft_in_rounds(ops, with_q):
-    """a batch whose rows are read in more than one round, sequences that end in each of them"""
-    target, tokens, u, E, draft = drafts(64, 8, 50021, torch.float32, 21, noise=0.1, scale=3.0)
-    lengths = (torch.arange(64) % 9).cuda()
-    lengths[::2] = 8
-    _, accepted = check_verify(ops, target, tokens if with_q else target[:, :8].argmax(-1), u if with_q else u * 0.3, E, draft if with_q else None, lengths)
-    assert len(set(accepted.tolist())) > 4
+    """a batch whose rows (320 MB) are read in more than one round, sequences that end in each of them"""
+    B, N, V = 64, 24, 50021
+    g = torch.Generator(device="cuda").manual_seed(3)
+    target = torch.randn(B, N + 1, V, generator=g, device="cuda") * 3
+    draft = target[:, :N] + torch.randn(B, N, V, generator=g, device="cuda") * 0.1
+    tokens = (draft - torch.empty_like(draft).exponential_(generator=g).log()).argmax(-1)       # drawn from softmax(draft)
+    u, E = torch.rand(B, N, generator=g, device="cuda"), torch.empty(B, V, device="cuda").exponential_(generator=g)
+    lengths = (torch.arange(B) % (N + 1)).cuda()
+    lengths[::2] = N
+    if with_q:
+        _, accepted = check_verify(ops, target, tokens, u, E, draft, lengths)
+    else:                                                                # the likeliest tokens, p around 0.1, against u below 0.05
+        _, accepted = check_verify(ops, target, target[:, :N].argmax(-1), u * 0.05, E, None, lengths)
+    assert (accepted < 5).any() and (accepted > 11).any() and len(set(accepted.tolist())) > 6
 
 
 # ------------------------------------------------------------------------------------------------
