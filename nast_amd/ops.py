@@ -1288,6 +1288,10 @@ class GeneratorDistillFn(torch.autograd.Function):
     def forward(ctx, x, W, b, temperature, top, tail):
         _chk(x, W, b)
         teacher = _teacher_list(x.shape[:-1], top, temperature, tail)
+        if W.dim() != 2 or W.shape[1] != x.shape[-1] or (b is not None and b.shape != W.shape[:1]):
+            raise _lib.NastHipError(f"weight {tuple(W.shape)} and bias {None if b is None else tuple(b.shape)} for rows of {x.shape[-1]}")
+        if not W.is_contiguous() or (b is not None and not b.is_contiguous()):
+            raise _lib.NastHipError("contiguous weight and bias expected")
         stream = _on_device(x, W, b, *teacher)
         x2 = _c(x).view(-1, x.shape[-1])
         V = W.shape[0]
