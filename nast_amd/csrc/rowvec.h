@@ -231,10 +231,11 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 }
 
 // Into how many chunks a row of V elements is cut: as few as `most` elements a chunk allow; more while rows * chunks is below 512
-// workgroups (two a compute unit), but none shorter than `least`.
-static inline int row_chunks(int rows, int V, int most, int least) {
+// workgroups (two a compute unit), but none shorter than `least`.  Chunks of ceil(V / n) elements then leave none empty, as long as
+// n * n <= V: `least` and `most` here are 2048 and more, n is 512 and less.
+static inline int row_chunks(int64_t rows, int V, int most, int least) {
   const int need = (V + most - 1) / most;
-  int n = rows > 0 && rows < 512 ? (512 + rows - 1) / rows : 1;
+  int n = rows > 0 && rows < 512 ? (int)((512 + rows - 1) / rows) : 1;
   if (n > V / least) n = V / least;
   return n > need ? n : need;
 }

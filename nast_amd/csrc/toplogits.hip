@@ -75,7 +75,7 @@ __device__ __forceinline__ void group_bound(const float* gmax, int kk, float* bo
   m = wave_max(m);
   least = -wave_max(-least);
   uint32_t b0 = order_key(least) >> 16, b1 = (order_key(m) >> 16) + 1;
-  while (b1 - b0 > 1) {
+  while (b0 + 1 < b1) {                                        // (false at once where nothing but signalling NaNs came: least > m)
     const uint32_t mid = (b0 + b1) >> 1;
     int n = 0;
 #pragma unroll
@@ -106,8 +106,9 @@ struct TopPart {
 // maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and one
 // wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to LDS, each wavefront's to a place of
 // its own, where its lanes look at their elements one by one; what reaches the bound (a little more than k elements where they lie at
-// random) is ranked by counting.  Where more than TOP_WAVE elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the
-// registers, and equal elements are taken in the order of their ids.
+// random) is ranked by counting.  Where more than TOP_WAVE elements of a wavefront reach it (many equal values, e.g. a constant row), or
+// the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are taken in
+// the order of their ids.
 template <class D, int NV>
 __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
       return block_count<256>(q, cnt);
     };
     uint64_t b0 = 0, b1 = 1ull << (32 - SHIFT);
-    while (b1 - b0 > 1) {
+    while (b0 + 1 < b1) {
       const uint64_t mid = (b0 + b1) >> 1;
       if (count(mid) >= kk) b0 = mid;
       else b1 = mid;
@@ -348,18 +349,23 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
 #pragma unroll
   for (int i = 0; i < 16; ++i) o[i] = i * NT + (int)threadIdx.x < n ? lists[r * n + i * NT + threadIdx.x] : 0;
   if (threadIdx.x == 0) n_cand = 0;
-  // at least k entries reach the largest of the chunks' bounds
+  // At least k entries reach the largest of the chunks' bounds, none lies above the largest maximum: where every chunk has a bound.
+  // Else (a NaN somewhere, many equal values) b0 = 1 is below all entries and b1 not below the largest.
   float bound = -INFINITY, top = -INFINITY;
+  bool known = true;
   for (int i = threadIdx.x & 63; i < n_chunk; i += 64) {
-    bound = fmaxf(bound, parts[r * n_chunk + i].bound);
-    top = fmaxf(top, (float)parts[r * n_chunk + i].m);
+    const TopPart q = parts[r * n_chunk + i];
+    known = known && q.bound > -INFINITY;
+    bound = fmaxf(bound, q.bound);
+    top = fmaxf(top, (float)q.m);
   }
   bound = wave_max(bound);
   top = wave_max(top);
-  uint64_t b0 = bound > -INFINITY ? (uint64_t)order_key(bound) << 32 : 1;
+  known = __ballot(!known) == 0;
+  uint64_t b0 = known ? (uint64_t)order_key(bound) << 32 : 1;
   if (n > k + k / 4 + 32) {
-    uint64_t b1 = bound > -INFINITY ? (uint64_t)(order_key(top) + 1) << 32 : ~0ull;   // above all entries, or not below the largest
-    while (b1 - b0 > 1) {
+    uint64_t b1 = known ? ((uint64_t)order_key(top) + 1) << 32 : ~0ull;
+    while (b0 + 1 < b1) {
       const uint64_t mid = b0 + ((b1 - b0) >> 1);
       int q = 0;
 #pragma unroll

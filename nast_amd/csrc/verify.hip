@@ -392,7 +392,7 @@ static int verify_round(const VerifyArgs& A, int dtype, int i0, int last) {
 // 16 x 8 drafts x 50021 fp16 29 us in one workgroup, 25 in chunks; 32000 bf16 the same either way).
 static void verify_plan(VerifyArgs& A, int dtype) {
   const int most = 1 << 15, first = verify_round(A, dtype, 0, 1);
-  A.n_chunk = row_chunks(A.B * first * (A.draft ? 2 : 1), A.V, most, 1 << 13);
+  A.n_chunk = row_chunks((int64_t)A.B * first * (A.draft ? 2 : 1), A.V, most, 1 << 13);
   A.chunk = (A.V + A.n_chunk - 1) / A.n_chunk;
   A.n_race = A.V <= most ? 1 : row_chunks(A.B, A.V, most, 1 << 13);
   A.race_chunk = (A.V + A.n_race - 1) / A.n_race;

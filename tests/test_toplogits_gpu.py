@@ -120,6 +120,21 @@ def test_top_logits_largest(ops, dtype):
     check_top(ops, x, k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_top_logits_nans_in_one_chunk(ops, dtype):
+    """chunks that go different ways: NaNs in one (more of them than the join keeps), equal values in another, signalling NaNs alone"""
+    V = 70001
+    for k in (1, 64, 256):
+        x = rows(4, V, dtype, k)
+        x[0, :5000] = float("nan")
+        x[1, 40000:] = 1.25
+        x[2, 30000:30003] = float("nan")
+        kind = torch.int32 if dtype == torch.float32 else torch.int16
+        x[3] = torch.full((V,), {torch.float32: 0x7fa00000, torch.bfloat16: 0x7fa0, torch.float16: 0x7d00}[dtype], dtype=kind, device="cuda").view(dtype)
+        check_top(ops, x, k)
+        check_top(ops, x[:, :1500], k)
+
+
 def test_top_logits_far_offsets(ops):
     """rows that lie beyond 2^31 elements of their tensor"""
     R, V = 20000, 120000
@@ -362,6 +377,20 @@ def test_top_distill_differences(ops):
             h = (a[0, e] - b[0, e]).item()
             d = (ops.top_distill(a, top, 1.3, tail=tail) - ops.top_distill(b, top, 1.3, tail=tail)).item() / h
             assert abs(d - leaf.grad[0, e].item()) < 1e-4
+
+
+def test_generator_distill_refusals_and_no_rows(ops):
+    top = ops.TopLogits(torch.zeros(2, 3, device="cuda"), torch.zeros(2, 3, device="cuda", dtype=torch.int64), None, 1.0)
+    x, W, b = torch.randn(2, 16, device="cuda"), torch.randn(40, 16, device="cuda"), torch.zeros(40, device="cuda")
+    for bad in ((x, W[:, :8].contiguous(), b), (x, W, b[:39]), (x, W[:, ::2], b), (x, W.t().contiguous().t(), b), (x[:1], W, b), (x.half(), W, b)):
+        with pytest.raises(ops._lib.NastHipError):
+            ops.generator_distill(*bad, 1.0, top)
+    none = ops.TopLogits(top.values[:0], top.index[:0], None, 1.0)
+    leaves = [t.clone().requires_grad_() for t in (x[:0], W, b)]
+    loss = ops.generator_distill(*leaves, 1.0, none)
+    assert loss.shape == (0,)
+    loss.sum().backward()
+    assert all(t.grad is None or not t.grad.any() for t in leaves)
 
 
 def test_generator_top_and_distill(ops):
