@@ -37,7 +37,7 @@ struct VerifyBest {
   float score, lower, upper, other;
   int at;
 };
-__device__ __forceinline__ void best_merge(VerifyBest& a, const VerifyBest& b) {
+__device__ __forceinline__ void best_merge(VerifyBest& a, const VerifyBest b) {
   const float other = fmaxf(a.other, b.other);
   if (b.score > a.score || (b.score == a.score && b.at < a.at)) {
     const float beaten = a.upper;
@@ -67,11 +67,17 @@ __device__ __forceinline__ MaxSumD proper(MaxSumD t) {
   return t;
 }
 
-// a row's sum in double, by the whole workgroup
-template <class D, int NT>
+// a row's sum in double, by the whole workgroup; U loads in flight
+template <class D, int NT, int U>
 __device__ double row_sum_exact(const VerifyArgs& A, const typename D::store* p, double m, double* red) {
   double s = 0;
-  for (int e = threadIdx.x; e < A.V; e += NT) s += exp(((double)D::get(p[e]) - m) * A.it);
+  for (int e = threadIdx.x; e < A.V; e += U * NT) {
+    float z[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) z[i] = D::get(p[min(e + i * NT, A.V - 1)]);
+#pragma unroll
+    for (int i = 0; i < U; ++i) s += e + i * NT < A.V ? exp(((double)z[i] - m) * A.it) : 0.0;
+  }
   s = wave_sum_d(s);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -100,10 +106,10 @@ __device__ __forceinline__ bool too_close(const VerifyPair& r, float u) {
   return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= 1e-5 * r.p;   // (two sums)
 }
 // the same decision with sums in double, by the whole workgroup
-template <class D, int NT>
+template <class D, int NT, int U>
 __device__ bool stands_exact(const VerifyArgs& A, int b, int i, MaxSumD p, MaxSumD q, double* red) {
-  p.s = row_sum_exact<D, NT>(A, target_row<D>(A, b, i), p.m, red);
-  if (A.draft) q.s = row_sum_exact<D, NT>(A, draft_row<D>(A, b, i), q.m, red);
+  p.s = row_sum_exact<D, NT, U>(A, target_row<D>(A, b, i), p.m, red);
+  if (A.draft) q.s = row_sum_exact<D, NT, U>(A, draft_row<D>(A, b, i), q.m, red);
   return stands(drafted<D>(A, b, i, p, q), A.u[(int64_t)b * A.N + i]);
 }
 
@@ -150,7 +156,10 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
       const float ep = pv * __builtin_fmaf(fmaxf(tp, far), slope, VERIFY_REL), eq = q ? qv * __builtin_fmaf(fmaxf(tq, far), slope, VERIFY_REL) : 0.f;
       const float err = 1e-37f + (ep + eq);
       const float upper = (d + err) * inv;
-      if (upper > seen && e != w.one) best_merge(a, {d * inv, (d - err) * inv, upper, 0.f, e});
+      if (upper > seen && e != w.one) {
+        if (en >= FLT_MIN) best_merge(a, {d * inv, (d - err) * inv, upper, 0.f, e});
+        else a.other = INFINITY;                                  // no reciprocal in fp32: left to the draw in double
+      }
     };
     const RowSpan16<D> rs(p, lo, hi);
     const int e = rs.edge(threadIdx.x);
@@ -196,28 +205,46 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
   return r;
 }
 
-// The draw in double, ties to the lowest id.  Where nothing is left of p - q (rounding, u >= 1) it is made from p.
-template <class D, int NT>
-__device__ int race_exact(const VerifyArgs& A, int b, const VerifyDraw& w, double* red, int* ired) {
+// The draw in double, ties to the lowest id.  Where nothing is left of p - q (rounding, u >= 1) it is made from p.  `lower`: what the
+// best score reaches for certain; elements that fall short of it by the measure of race() are passed over.
+template <class D, int NT, int U>
+__device__ int race_exact(const VerifyArgs& A, int b, const VerifyDraw& w, float lower, double* red, int* ired) {
   if (w.p.s == 0) return -1;
   const typename D::store* p = target_row<D>(A, b, w.place);
   const typename D::store* q = w.minus_q ? draft_row<D>(A, b, w.place) : nullptr;
-  const double ps = row_sum_exact<D, NT>(A, p, w.p.m, red), qs = q ? row_sum_exact<D, NT>(A, q, w.q.m, red) : 1;
+  const float* E = A.E + (int64_t)b * A.V;
+  // (scores of p alone are compared without its sum)
+  const double ps = q ? row_sum_exact<D, NT, U>(A, p, w.p.m, red) : w.p.s, qs = q ? row_sum_exact<D, NT, U>(A, q, w.q.m, red) : 1;
+  const float pm = (float)w.p.m, log_s = -(float)log2(w.p.s);
   for (int whole = 0; whole < 2; ++whole) {
+    const float least = whole || !(lower > 0) ? -INFINITY : __builtin_amdgcn_logf(lower) - 0.01f;
     double best = 0;
     int at = 0x7fffffff;
-    for (int e = threadIdx.x; e < A.V; e += NT) {
-      double v = exp(((double)D::get(p[e]) - w.p.m) * A.it) / ps;
+    auto look = [&](float z, float en, int e) {
+      if (__builtin_fmaf(z - pm, A.c, log_s) - __builtin_amdgcn_logf(en) < least) return;
+      double v = exp(((double)z - w.p.m) * A.it) / ps;
       if (!whole) {
         if (q) v -= exp(((double)D::get(q[e]) - w.q.m) * A.it) / qs;
         if (e == w.one) v = 0;
       }
-      if (!(v > 0)) continue;
-      const double score = v / (double)A.E[(int64_t)b * A.V + e];
-      if (score > best) {
+      if (!(v > 0)) return;
+      const double score = v / (double)en;
+      if (score > best || (score == best && e < at)) {
         best = score;
         at = e;
       }
+    };
+    for (int e = threadIdx.x; e < A.V; e += U * NT) {
+      float z[U], en[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int at = min(e + i * NT, A.V - 1);
+        z[i] = D::get(p[at]);
+        en[i] = E[at];
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (e + i * NT < A.V) look(z[i], en[i], e + i * NT);
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -243,15 +270,6 @@ __device__ int race_exact(const VerifyArgs& A, int b, const VerifyDraw& w, doubl
     if (best > 0) return at;
   }
   return -1;
-}
-
-// the end of a sequence, by the whole workgroup
-template <class D, int NT>
-__device__ void finish(const VerifyArgs& A, int b, const VerifyDraw& w, const VerifyBest& a, double* red, int* ired) {
-  const int token = a.lower > a.other ? a.at : race_exact<D, NT>(A, b, w, red, ired);
-  for (int i = threadIdx.x; i <= A.N; i += NT)
-    A.out[(int64_t)b * (A.N + 1) + i] = i < w.place ? A.tokens[(int64_t)b * A.N + i] : i == w.place ? token : -1;
-  if (threadIdx.x == 0) A.accepted[b] = w.place;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -312,8 +330,9 @@ __global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A, int
 }
 
 // How many drafts of sequence b stand, by the whole workgroup.  Each wavefront does the same: lane = place.  (Sums behind a clear refusal
-// may never have been written; what is made of them is not looked at.)
-template <class D, int NT>
+// may never have been written; what is made of them is not looked at.)  A decision that comes too close is made in double, or, with
+// U = 0, the answer is -1.
+template <class D, int NT, int U>
 __device__ int places(const VerifyArgs& A, int b, int len, double* red) {
   const int lane = threadIdx.x & 63;
   for (int base = 0; base < len; base += 64) {
@@ -329,11 +348,15 @@ __device__ int places(const VerifyArgs& A, int b, int len, double* red) {
     while (close) {
       const int at = __ffsll((unsigned long long)close) - 1;
       if (no & ((1ull << at) - 1)) break;                  // a clear refusal comes first
-      close &= close - 1;
-      const int j = base + at;
-      const MaxSumD p = row_pair(A, b * (A.N + 1) + j), q = A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + j) : MaxSumD{0, 1};
-      const bool yes = stands_exact<D, NT>(A, b, j, p, q, red);
-      no = yes ? no & ~(1ull << at) : no | (1ull << at);
+      if constexpr (U == 0) {
+        return -1;
+      } else {
+        close &= close - 1;
+        const int j = base + at;
+        const MaxSumD p = row_pair(A, b * (A.N + 1) + j), q = A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + j) : MaxSumD{0, 1};
+        const bool yes = stands_exact<D, NT, U>(A, b, j, p, q, red);
+        no = yes ? no & ~(1ull << at) : no | (1ull << at);
+      }
     }
     if (no) return base + __ffsll((unsigned long long)no) - 1;
   }
@@ -346,35 +369,58 @@ __device__ __forceinline__ VerifyDraw draw_at(const VerifyArgs& A, int b, int pl
                  A.draft && place < len ? row_pair(A, A.B * (A.N + 1) + b * A.N + place) : MaxSumD{0, 0});
 }
 
+// the end of a sequence, by the whole workgroup
+template <class D, int NT, int U>
+__device__ void finish(const VerifyArgs& A, int b, int place, int len, const VerifyBest& a, double* red, int* ired) {
+  const int token = a.lower > a.other ? a.at : race_exact<D, NT, U>(A, b, draw_at<D>(A, b, place, len), a.lower, red, ired);
+  for (int i = threadIdx.x; i <= A.N; i += NT)
+    A.out[(int64_t)b * (A.N + 1) + i] = i < place ? A.tokens[(int64_t)b * A.N + i] : i == place ? token : -1;
+  if (threadIdx.x == 0) A.accepted[b] = place;
+}
+
+// One workgroup a sequence does everything.
 template <class D, int NT>
 __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
   __shared__ double red[NT / 64];
   __shared__ int ired[NT / 64];
   __shared__ VerifyBest lds[NT / 64];
-  const int b = blockIdx.x / A.n_race, lo = (int)(blockIdx.x % A.n_race) * A.race_chunk, hi = min(A.V, lo + A.race_chunk);
-  const int len = draft_length(A, b), place = places<D, NT>(A, b, len, red);
-  const VerifyDraw w = draw_at<D>(A, b, place, len);
-  const VerifyBest a = race<D, NT>(A, b, w, lo, hi, lds);
-  if (A.n_race == 1) {
-    finish<D, NT>(A, b, w, a, red, ired);
-  } else if (threadIdx.x == 0) {
-    A.best[blockIdx.x] = a;
-    if (lo == 0) A.accepted[b] = place;
-  }
+  const int b = blockIdx.x, len = draft_length(A, b), place = places<D, NT, 1>(A, b, len, red);
+  finish<D, NT, 1>(A, b, place, len, race<D, NT>(A, b, draw_at<D>(A, b, place, len), 0, A.V, lds), red, ired);
 }
 
-// (1024 threads for the draw in double that it may have to make)
+// One workgroup a chunk of a sequence.  Decisions that are too close are left to the join: the arithmetic in double would cost this
+// kernel, which has to fill the card, 22 registers and three of eight wavefronts.  (Where one of 256 x 131072 comes too close, about
+// one call in a hundred, the call takes 130 us more.)
+template <class D>
+__global__ __launch_bounds__(256) void nast_verify_chunk_kernel(VerifyArgs A) {
+  __shared__ VerifyBest lds[4];
+  const int b = blockIdx.x / A.n_race, lo = (int)(blockIdx.x % A.n_race) * A.race_chunk, hi = min(A.V, lo + A.race_chunk);
+  const int len = draft_length(A, b), place = places<D, 256, 0>(A, b, len, nullptr);
+  if (place >= 0) {
+    const VerifyBest a = race<D, 256>(A, b, draw_at<D>(A, b, place, len), lo, hi, lds);
+    if (threadIdx.x == 0) A.best[blockIdx.x] = a;
+  }
+  if (lo == 0 && threadIdx.x == 0) A.accepted[b] = place;
+}
+
 template <class D>
 __global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
   __shared__ double red[16];
   __shared__ int ired[16];
-  const int b = blockIdx.x, len = draft_length(A, b), place = (int)A.accepted[b];
-  VerifyBest a = A.best[(int64_t)b * A.n_race];
-  for (int i = 1; i < A.n_race; ++i) best_merge(a, A.best[(int64_t)b * A.n_race + i]);
-  VerifyDraw w{};
-  w.place = place;
-  if (!(a.lower > a.other)) w = draw_at<D>(A, b, place, len);
-  finish<D, 1024>(A, b, w, a, red, ired);
+  __shared__ VerifyBest lds[16];
+  const int b = blockIdx.x, len = draft_length(A, b);
+  int place = (int)A.accepted[b];
+  VerifyBest a{0.f, 0.f, 0.f, 0.f, 0x7fffffff};
+  if (place >= 0) {
+    for (int i = 0; i < A.n_race; ++i) {
+      const VerifyBest o = A.best[(int64_t)b * A.n_race + i];
+      best_merge(a, o);
+    }
+  } else {
+    place = places<D, 1024, 4>(A, b, len, red);
+    a = race<D, 1024>(A, b, draw_at<D>(A, b, place, len), 0, A.V, lds);
+  }
+  finish<D, 1024, 4>(A, b, place, len, a, red, ired);
 }
 
 // A further round costs two launches (10 us) and saves the rows of the sequences that have ended, half of them perhaps: it has to have
@@ -462,7 +508,7 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
     if (A.n_race == 1) {
       hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
     } else {
-      hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B * A.n_race), dim3(256), 0, s, A);
+      hipLaunchKernelGGL((nast_verify_chunk_kernel<D>), dim3(B * A.n_race), dim3(256), 0, s, A);
       hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(1024), 0, s, A);
     }
   });

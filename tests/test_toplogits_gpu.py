@@ -527,6 +527,41 @@ def test_verify_draft_borders(ops, dtype, V):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [64, 40000])
+def test_verify_draft_borders_many_places(ops, dtype, V):
+    """a ratio of 1/2 at every place: u next to it decides, place after place, clear decisions between"""
+    N = 70
+    target = torch.zeros(5, N + 1, V, dtype=dtype, device="cuda")
+    draft = torch.zeros(5, N, V, dtype=dtype, device="cuda")
+    draft[:, :, V // 2:] = -INF
+    tokens = torch.arange(N, device="cuda").remainder(V // 2).expand(5, N)
+    below = float(torch.nextafter(torch.tensor(0.5), torch.tensor(0.0)))
+    u = torch.full((5, N), below, device="cuda")
+    u[1, 68], u[2, 3], u[2, 2], u[3, :66], u[4, 66] = 0.5, 0.5, 0.9, 0.1, 0.5
+    E = torch.rand(5, V, generator=torch.Generator().manual_seed(3)).add(0.5).cuda()
+    _, accepted = check_verify(ops, target, tokens, u, E, draft)
+    assert accepted.tolist() == [70, 68, 2, 70, 66]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [600, 40000])
+def test_verify_draft_smallest_draws(ops, dtype, V):
+    """Exp(1) draws below the smallest normal number (their reciprocal has no fp32), zeros, infinities, the largest number"""
+    target, tokens, u, E, draft = drafts(6, 2, V, dtype, 21, noise=0.5)
+    at = torch.tensor([V - 1, 7, 311], device="cuda")
+    E[0, at] = torch.tensor([1e-40, 2e-40, 3e-45], device="cuda")
+    E[1, at] = torch.tensor([1e-40, 1.3e-38, 1e-37], device="cuda")
+    E[2, at] = torch.tensor([0.0, 0.0, 1e-44], device="cuda")
+    E[3] = 1e-42
+    E[4, at] = INF
+    E[5] = torch.finfo(torch.float32).max
+    for t in (1.0, 0.05):
+        check_verify(ops, target, tokens, u, E, draft, None, t)
+        check_verify(ops, target, tokens, u * 0 + 2, E, draft, None, t)
+        check_verify(ops, target, tokens, u, E, None, None, t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_verify_draft_strides(ops, dtype):
     target, tokens, u, E, draft = drafts(6, 5, 301, dtype, 4)
     check_verify(ops, target[::2, 1:, 3:], tokens[::2, 1:].clamp(max=297), u[::2, 1:], E[::2, 3:], draft[::2, 1:, 3:])
