@@ -132,9 +132,22 @@ __device__ __forceinline__ VerifyDraw draw_of(const VerifyArgs& A, int b, int pl
   return w;
 }
 
+// the best of the wavefront's, in every lane.  (Of equal scores any: neither is certain then.)
+__device__ __forceinline__ VerifyBest best_of_wave(const VerifyBest& a) {
+  VerifyBest r;
+  r.score = wave_max(a.score);
+  const int l = __ffsll((unsigned long long)__ballot(a.score == r.score)) - 1;
+  r.lower = __shfl(a.lower, l, 64);
+  r.upper = __shfl(a.upper, l, 64);
+  r.at = __shfl(a.at, l, 64);
+  r.other = wave_max((threadIdx.x & 63) == l ? a.other : fmaxf(a.other, a.upper));
+  return r;
+}
+
 // Argmax of w / E over [lo, hi) in fp32 with error bounds, by the whole workgroup.  Most elements are told apart by one logarithm:
 // log2(p / E), not less than the logarithm of their score, against that of the best lower bound their wavefront has seen (less 0.01, a
-// thousand times what the two are off by).  Only what passes is looked at closer.
+// thousand times what the two are off by).  Only what passes is looked at closer, and of the first vectors, where nothing has been seen
+// yet, each lane's most promising element before the others.
 template <class D, int NT>
 __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int lo, int hi, VerifyBest* lds) {
   VerifyBest a{0.f, 0.f, 0.f, 0.f, 0x7fffffff};
@@ -146,10 +159,9 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     const float slope = -VERIFY_REL_EXP * A.c, far = -200.f / A.c;
     float seen = 0.f;
     float seen_log = -INFINITY;
+    auto log_score = [&](float zp, float en) { return __builtin_fmaf(zp - pm, A.c, ps) - __builtin_amdgcn_logf(en); };
     auto look = [&](float zp, float zq, float en, int e) {
-      const float tp = zp - pm, log_p = __builtin_fmaf(tp, A.c, ps);
-      if (log_p - __builtin_amdgcn_logf(en) < seen_log) return;   // (a draw of 0 or NaN passes)
-      const float tq = zq - qm, pv = __builtin_amdgcn_exp2f(log_p);
+      const float tp = zp - pm, tq = zq - qm, pv = __builtin_amdgcn_exp2f(__builtin_fmaf(tp, A.c, ps));
       const float qv = q ? __builtin_amdgcn_exp2f(__builtin_fmaf(tq, A.c, qs)) : 0.f;
       const float d = pv - qv, inv = __builtin_amdgcn_rcpf(en);
       // (below 2^-150 the bound is the absolute one; an exponent of -inf would make it 0 * inf)
@@ -162,8 +174,8 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
       }
     };
     const RowSpan16<D> rs(p, lo, hi);
-    const int e = rs.edge(threadIdx.x);
-    if (e >= 0) look(D::get(p[e]), q ? D::get(q[e]) : 0.f, E[e], e);
+    const int edge = rs.edge(threadIdx.x), at_edge = edge >= 0 ? edge : lo;
+    const float edge_p = D::get(p[at_edge]), edge_q = D::get((q ? q : p)[at_edge]), edge_E = E[at_edge];
     constexpr int U = 2, W = D::EPV / 4;                        // W: vectors of draws to one of logits
     for (int b0 = 0; b0 < rs.n; b0 += NT * U) {
       RowVec<D> pv[U], qv[U];
@@ -178,31 +190,43 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
       }
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        seen = wave_max(fmaxf(seen, a.lower));                  // (every lane takes part)
-        seen_log = __builtin_amdgcn_logf(seen) - 0.01f;
         const int s = b0 + NT * i + (int)threadIdx.x;
-        if (s < rs.n)
+        float sc[D::EPV], top = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < D::EPV; ++j) look(pv[i].get(j), qv[i].get(j), ev[i][j / 4].get(j % 4), rs.elem(s) + j);
+        for (int j = 0; j < D::EPV; ++j) {                      // (a draw of 0: +inf; NaN for one that never wins)
+          sc[j] = log_score(pv[i].get(j), ev[i][j / 4].get(j % 4));
+          top = fmaxf(top, sc[j]);
+        }
+        const bool hit = s < rs.n && top > -INFINITY && top >= seen_log;
+        if (!__ballot(hit)) continue;
+        int first = 0;
+        if (hit) {
+          float zp = 0.f, zq = 0.f, en = 1.f;
+#pragma unroll
+          for (int j = D::EPV - 1; j >= 0; --j) {
+            const bool is = sc[j] == top;
+            zp = is ? pv[i].get(j) : zp;
+            zq = is ? qv[i].get(j) : zq;
+            en = is ? ev[i][j / 4].get(j % 4) : en;
+            first = is ? j : first;
+          }
+          look(zp, zq, en, rs.elem(s) + first);
+        }
+        seen = wave_max(fmaxf(seen, a.lower));
+        seen_log = __builtin_amdgcn_logf(seen) - 0.01f;
+        if (hit)
+#pragma unroll
+          for (int j = 0; j < D::EPV; ++j)
+            if (sc[j] >= seen_log && j != first) look(pv[i].get(j), qv[i].get(j), ev[i][j / 4].get(j % 4), rs.elem(s) + j);
       }
     }
+    if (edge >= 0 && log_score(edge_p, edge_E) >= seen_log) look(edge_p, edge_q, edge_E, edge);
   }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    VerifyBest x;
-    x.score = __shfl_xor(a.score, o, 64);
-    x.lower = __shfl_xor(a.lower, o, 64);
-    x.upper = __shfl_xor(a.upper, o, 64);
-    x.other = __shfl_xor(a.other, o, 64);
-    x.at = __shfl_xor(a.at, o, 64);
-    best_merge(a, x);
-  }
+  a = best_of_wave(a);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
   __syncthreads();
-  VerifyBest r = lds[0];
-  for (int i = 1; i < NT / 64; ++i) best_merge(r, lds[i]);
-  return r;
+  return best_of_wave((threadIdx.x & 63) < NT / 64 ? lds[threadIdx.x & 63] : VerifyBest{0.f, 0.f, 0.f, 0.f, 0x7fffffff});
 }
 
 // The draw in double, ties to the lowest id.  Where nothing is left of p - q (rounding, u >= 1) it is made from p.  `lower`: what the
