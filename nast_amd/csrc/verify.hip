@@ -176,48 +176,55 @@ __device__ VerifyBest race(const VerifyArgs& A, int b, const VerifyDraw& w, int 
     const RowSpan16<D> rs(p, lo, hi);
     const int edge = rs.edge(threadIdx.x), at_edge = edge >= 0 ? edge : lo;
     const float edge_p = D::get(p[at_edge]), edge_q = D::get((q ? q : p)[at_edge]), edge_E = E[at_edge];
-    constexpr int U = 2, W = D::EPV / 4;                        // W: vectors of draws to one of logits
-    for (int b0 = 0; b0 < rs.n; b0 += NT * U) {
-      RowVec<D> pv[U], qv[U];
-      RowVec<RowF32> ev[U][W];
+    constexpr int W = D::EPV / 4;                               // vectors of draws to one of logits
+    struct Slot {
+      RowVec<D> p, q;
+      RowVec<RowF32> E[W];
+    };
+    auto load = [&](int s) {
+      const int at = rs.elem(min(s, rs.n - 1));
+      Slot v;
+      v.p = vec_load<D>(p + at);
+      v.q = vec_load_any<D>((q ? q : p) + at);
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int at = rs.elem(min(b0 + NT * i + (int)threadIdx.x, rs.n - 1));
-        pv[i] = vec_load<D>(p + at);
-        qv[i] = vec_load_any<D>((q ? q : p) + at);
-#pragma unroll
-        for (int j = 0; j < W; ++j) ev[i][j] = vec_load_any<RowF32>(E + at + 4 * j);
-      }
-#pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int s = b0 + NT * i + (int)threadIdx.x;
-        float sc[D::EPV], top = -INFINITY;
+      for (int j = 0; j < W; ++j) v.E[j] = vec_load_any<RowF32>(E + at + 4 * j);
+      return v;
+    };
+    if (rs.n > 0) {
+      Slot v = load(threadIdx.x);
+#pragma unroll 1
+      for (int b0 = 0; b0 < rs.n; b0 += NT) {
+        const int s = b0 + (int)threadIdx.x;
+        const Slot next = load(s + NT);
+        float sc[D::EPV];
 #pragma unroll
         for (int j = 0; j < D::EPV; ++j) {                      // (a draw of 0: +inf; NaN for one that never wins)
-          sc[j] = log_score(pv[i].get(j), ev[i][j / 4].get(j % 4));
-          top = fmaxf(top, sc[j]);
+          sc[j] = log_score(v.p.get(j), v.E[j / 4].get(j % 4));
+          if (s >= rs.n) sc[j] = -INFINITY;
         }
-        const bool hit = s < rs.n && top > -INFINITY && top >= seen_log;
-        if (!__ballot(hit)) continue;
-        int first = 0;
-        if (hit) {
+#pragma unroll 1
+        while (true) {                                          // each lane's most promising element, as long as any lane has one
+          float top = sc[0];
+#pragma unroll
+          for (int j = 1; j < D::EPV; ++j) top = fmaxf(top, sc[j]);
+          const bool hit = top > -INFINITY && top >= seen_log;
+          if (!__ballot(hit)) break;
           float zp = 0.f, zq = 0.f, en = 1.f;
+          int first = -1;
 #pragma unroll
-          for (int j = D::EPV - 1; j >= 0; --j) {
-            const bool is = sc[j] == top;
-            zp = is ? pv[i].get(j) : zp;
-            zq = is ? qv[i].get(j) : zq;
-            en = is ? ev[i][j / 4].get(j % 4) : en;
+          for (int j = 0; j < D::EPV; ++j) {
+            const bool is = first < 0 && sc[j] == top;
+            zp = is ? v.p.get(j) : zp;
+            zq = is ? v.q.get(j) : zq;
+            en = is ? v.E[j / 4].get(j % 4) : en;
             first = is ? j : first;
+            sc[j] = is ? -INFINITY : sc[j];
           }
-          look(zp, zq, en, rs.elem(s) + first);
+          if (hit) look(zp, zq, en, rs.elem(s) + first);
+          seen = wave_max(fmaxf(seen, a.lower));
+          seen_log = __builtin_amdgcn_logf(seen) - 0.01f;
         }
-        seen = wave_max(fmaxf(seen, a.lower));
-        seen_log = __builtin_amdgcn_logf(seen) - 0.01f;
-        if (hit)
-#pragma unroll
-          for (int j = 0; j < D::EPV; ++j)
-            if (sc[j] >= seen_log && j != first) look(pv[i].get(j), qv[i].get(j), ev[i][j / 4].get(j % 4), rs.elem(s) + j);
+        v = next;
       }
     }
     if (edge >= 0 && log_score(edge_p, edge_E) >= seen_log) look(edge_p, edge_q, edge_E, edge);
@@ -458,8 +465,8 @@ static int verify_round(const VerifyArgs& A, int dtype, int i0, int last) {
   const int64_t n = least > 2 * last ? least : 2 * last;
   return n + least >= left ? left : (int)n;
 }
-// Chunks: rows at most 2^15 elements, the draw up to there in one workgroup of 1024 (a join of its own costs as much as that takes:
-// 16 x 8 drafts x 50021 fp16 29 us in one workgroup, 25 in chunks; 32000 bf16 the same either way).
+// Chunks: rows at most 2^15 elements, the draw up to there in one workgroup (a join of its own costs more than chunks save: 1 x 4 drafts x
+// 32000 bf16 17.8 us in one workgroup, 20.3 in chunks; 100 x 2 x 30000 22 either way).
 static void verify_plan(VerifyArgs& A, int dtype) {
   const int most = 1 << 15, first = verify_round(A, dtype, 0, 1);
   A.n_chunk = row_chunks((int64_t)A.B * first * (A.draft ? 2 : 1), A.V, most, 1 << 13);
@@ -530,7 +537,9 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
       hipLaunchKernelGGL((nast_verify_rows_kernel<D>), dim3(B * (n + n_draft) * A.n_chunk), dim3(256), 0, s, A, i0, n, n_draft);
     }
     if (A.n_race == 1) {
-      hipLaunchKernelGGL((nast_verify_draw_kernel<D, 1024>), dim3(B), dim3(1024), 0, s, A);
+      // (512 threads where the workgroups do not fill the card twice: 128 x 9600 fp32 27 us, with 256 threads 29; 600 x 30000 bf16 67 and 60)
+      if (B <= 512) hipLaunchKernelGGL((nast_verify_draw_kernel<D, 512>), dim3(B), dim3(512), 0, s, A);
+      else hipLaunchKernelGGL((nast_verify_draw_kernel<D, 256>), dim3(B), dim3(256), 0, s, A);
     } else {
       hipLaunchKernelGGL((nast_verify_chunk_kernel<D>), dim3(B * A.n_race), dim3(256), 0, s, A);
       hipLaunchKernelGGL((nast_verify_join_kernel<D>), dim3(B), dim3(1024), 0, s, A);

@@ -1246,6 +1246,12 @@ def _distill_bwd(g, x, r, rows, dtype, values, index, stats, temperature, stream
     return gx
 
 
+def _once(backward):
+    """once_differentiable, whose checks take 5 us of the host, only where a backward pass records a graph of its own."""
+    checked = once_differentiable(backward)
+    return lambda ctx, g: checked(ctx, g) if torch.is_grad_enabled() else backward(ctx, g)
+
+
 class TopDistillFn(torch.autograd.Function):
     """KL(teacher || student) per row, the teacher known by its top logits; one pass over the logits each way."""
 
@@ -1261,7 +1267,7 @@ class TopDistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         x, values, index, stats = ctx.saved_tensors
         r, rows, dtype, temperature = ctx.call
@@ -1305,7 +1311,7 @@ class GeneratorDistillFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         x2, W, y, values, index, stats = ctx.saved_tensors
         gl = _distill_bwd(_c(g), y, Rows(W.shape[0], 0, 0), y.shape[0], 0, values, index, stats, ctx.temperature, _on_device(y, g))
