@@ -20,28 +20,14 @@
 __device__ __forceinline__ uint64_t top_entry(float f, int e) { return ((uint64_t)order_key(f) << 32) | (uint32_t)~e; }
 __device__ __forceinline__ int entry_id(uint64_t o) { return (int)~(uint32_t)o; }
 
-// Distinct entries in LDS, n[g] of them at cand + g * STRIDE: each goes to out(rank among all, entry) where the rank is below k.  A rank
-// is a count of larger entries.
-template <int NT, int GROUPS, int STRIDE, class F>
-__device__ __forceinline__ void rank_out(const uint64_t* cand, const int (&n)[GROUPS], int k, F&& out) {
-  int all = 0;
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) all += n[g];
-  for (int i = threadIdx.x; i < all; i += NT) {
-    int at = i, g = 0;
-#pragma unroll
-    for (int h = 0; h < GROUPS - 1; ++h)
-      if (g == h && at >= n[h]) {
-        at -= n[h];
-        ++g;
-      }
-    const uint64_t o = cand[g * STRIDE + at];
+// n distinct entries in LDS: each goes to out(rank among all, entry) where the rank is below k.  A rank is a count of larger entries.
+template <int NT, class F>
+__device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, F&& out) {
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t o = cand[i];
     int rank = 0;
-#pragma unroll
-    for (int h = 0; h < GROUPS; ++h) {
 #pragma unroll 4
-      for (int j = 0; j < n[h]; ++j) rank += cand[h * STRIDE + j] > o ? 1 : 0;
-    }
+    for (int j = 0; j < n; ++j) rank += cand[j] > o ? 1 : 0;
     if (rank < k) out(rank, o);
   }
 }
@@ -100,7 +86,8 @@ struct TopPart {
   float bound;
 };
 
-// One workgroup per chunk of a row, the chunk in registers: NV vectors a thread (and an edge element), read from memory once.
+// One workgroup of NT threads per chunk of a row, the chunk in registers: NV vectors a thread (and an edge element), read from memory
+// once.
 //
 // The k-th largest of the maxima of disjoint groups of elements is a lower bound of the k-th largest element.  Each thread keeps the
 // maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and one
@@ -109,19 +96,19 @@ struct TopPart {
 // random) is ranked by counting.  Where more than TOP_WAVE elements of a wavefront reach it (many equal values, e.g. a constant row), or
 // the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are taken in
 // the order of their ids.
-template <class D, int NV>
-__global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
+template <class D, int NT, int NV>
+__global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
                                                              float* __restrict__ lse, uint64_t* __restrict__ lists,
                                                              TopPart* __restrict__ parts, int V, int k, int len, int chunk, int n_chunk,
                                                              double inv_temp, float c) {
-  constexpr int G = NV >= 4 ? 4 : 1;
-  __shared__ float gmax[256 * G];
-  __shared__ uint64_t cand[4 * TOP_WAVE];
-  __shared__ uint4 vec_data[4 * TOP_WAVE];
-  __shared__ int vec_slot[4 * TOP_WAVE];
-  __shared__ double red[4];
-  __shared__ int cnt[4];
+  constexpr int W = NT / 64, G = NT == 256 && NV >= 4 ? 4 : 1;
+  __shared__ float gmax[NT * G];
+  __shared__ uint64_t cand[W * TOP_WAVE];
+  __shared__ uint4 vec_data[W * TOP_WAVE];
+  __shared__ int vec_slot[W * TOP_WAVE];
+  __shared__ double red[W];
+  __shared__ int cnt[W];
   __shared__ float bound[2];
   __shared__ int n_cand;
   const int64_t r = blockIdx.x / n_chunk;
@@ -135,14 +122,14 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   // (no branch around a single load: the compiler would wait for each before the next)
   if (rs.n > 0) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) v[i] = rs.load(p, min(i * 256 + tid, rs.n - 1));
+    for (int i = 0; i < NV; ++i) v[i] = rs.load(p, min(i * NT + tid, rs.n - 1));
   } else {
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = vec_of<D>(-INFINITY);
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
-    if ((i + 1) * 256 > rs.n && i * 256 + tid >= rs.n) v[i] = vec_of<D>(-INFINITY);
+    if ((i + 1) * NT > rs.n && i * NT + tid >= rs.n) v[i] = vec_of<D>(-INFINITY);
   const float ef = ee >= 0 ? D::get(edge) : -INFINITY;
 
   float vm[NV], g[G];
@@ -164,7 +151,7 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   const int groups = G > 1 && k > 64 ? G : 1;
   if (groups > 1) {
 #pragma unroll
-    for (int i = 0; i < G; ++i) gmax[i * 256 + tid] = g[i];
+    for (int i = 0; i < G; ++i) gmax[i * NT + tid] = g[i];
   } else {
 #pragma unroll
     for (int i = 1; i < G; ++i) g[0] = fmaxf(g[0], g[i]);
@@ -173,8 +160,8 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   __syncthreads();
 
   if (tid < 64) {
-    if (groups > 1) group_bound<4 * G>(gmax, kk, bound);
-    else group_bound<4>(gmax, kk, bound);
+    if (groups > 1) group_bound<W * G>(gmax, kk, bound);
+    else group_bound<W>(gmax, kk, bound);
   }
   __syncthreads();
   const float thr = bound[0], m = bound[1];
@@ -184,12 +171,12 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   int n_vec = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const bool hit = vm[i] >= thr && i * 256 + tid < rs.n;
+    const bool hit = vm[i] >= thr && i * NT + tid < rs.n;
     const uint64_t all = __ballot(hit);
     if (all) {
       const int at = n_vec + lanes_below(all);
       if (hit && at < TOP_WAVE) {
-        vec_slot[w0 + at] = i * 256 + tid;
+        vec_slot[w0 + at] = i * NT + tid;
         vec_data[w0 + at] = make_uint4(v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]);
       }
       n_vec += __popcll(all);
@@ -199,7 +186,7 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
   float sum = exp_t(ef - m, c);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (i * 256 < rs.n) {
+    if (i * NT < rs.n) {
       float t = 0.f;
 #pragma unroll
       for (int j = 0; j < D::EPV; ++j) t += exp_t(v[i].get(j) - m, c);
@@ -236,20 +223,28 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
     cnt[tid >> 6] = max(n_own, n_vec);                          // (a vector that does not fit has an element that does not)
   }
   __syncthreads();
-  const double s = (red[0] + red[1]) + (red[2] + red[3]);
-  int n[4] = {cnt[0], cnt[1], cnt[2], cnt[3]};
+  double s = 0;
+  int all = 0, before_wave = 0, most = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    s += red[i];
+    before_wave += i < tid >> 6 ? cnt[i] : 0;
+    all += cnt[i];
+    most = max(most, cnt[i]);
+  }
 
-  const bool exact = s != s || max(max(n[0], n[1]), max(n[2], n[3])) > TOP_WAVE;
+  uint64_t* flat = (uint64_t*)vec_data;                         // the candidates without gaps
+  const bool exact = s != s || most > TOP_WAVE;
   if (exact) {                                 // (from memory again: a copy in registers would cost every row its place)
     constexpr int SHIFT = D::KEY_ZEROS;
     auto count = [&](uint64_t at_least) {                       // elements with key >> SHIFT at or above
       int q = ee >= 0 && (order_key(ef) >> SHIFT) >= at_least ? 1 : 0;
-      for (int s = tid; s < rs.n; s += 256) {
+      for (int s = tid; s < rs.n; s += NT) {
         const RowVec<D> w = rs.load(p, s);
 #pragma unroll
         for (int j = 0; j < D::EPV; ++j) q += (order_key(w.get(j)) >> SHIFT) >= at_least ? 1 : 0;
       }
-      return block_count<256>(q, cnt);
+      return block_count<NT>(q, cnt);
     };
     uint64_t b0 = 0, b1 = 1ull << (32 - SHIFT);
     while (b0 + 1 < b1) {
@@ -262,9 +257,9 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
     __syncthreads();
     int before = 0;
     // pieces of ascending ids: head, the vectors one row of slots after the other, tail
-    const int pieces = (rs.n + 255) / 256;
+    const int pieces = (rs.n + NT - 1) / NT;
     for (int piece = -1; piece <= pieces; ++piece) {
-      const int s = piece * 256 + tid;
+      const int s = piece * NT + tid;
       uint32_t same = 0, more = 0;
       RowVec<D> w = vec_of<D>(ef);                              // an edge element stands first
       if (piece == -1 || piece == pieces) {
@@ -293,7 +288,7 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
       __syncthreads();
       int place = before + scan - own;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < W; ++i) {
         if (i < tid >> 6) place += cnt[i];
         before += cnt[i];
       }
@@ -301,36 +296,34 @@ __global__ __launch_bounds__(256, 4) void nast_top_chunk_kernel(const typename D
       for (int j = 0; j < D::EPV; ++j) {
         const bool eq = same >> j & 1;
         if ((eq && place < need) || (more >> j & 1))
-          cand[atomicAdd(&n_cand, 1)] = top_entry(w.get(j), piece == -1 || piece == pieces ? ee : rs.elem(s) + j);
+          flat[atomicAdd(&n_cand, 1)] = top_entry(w.get(j), piece == -1 || piece == pieces ? ee : rs.elem(s) + j);
         place += eq ? 1 : 0;
       }
     }
+    all = kk;
     __syncthreads();
-    n[0] = kk;
-    n[1] = n[2] = n[3] = 0;
+  } else if (n_chunk == 1 || all > len) {
+    for (int i = lane; i < n_own; i += 64) flat[before_wave + i] = cand[w0 + i];
+    __syncthreads();
   }
 
   if (n_chunk == 1) {
-    rank_out<256, 4, TOP_WAVE>(cand, n, k, [&](int rank, uint64_t o) {
+    rank_out<NT>(flat, all, k, [&](int rank, uint64_t o) {
       index[r * k + rank] = entry_id(o);
       values[r * k + rank] = D::put(key_value((uint32_t)(o >> 32)));
     });
-    if (tid == 0) lse[r] = (float)((double)m * inv_temp + logf((float)s));
+    if (tid == NT - 1) lse[r] = (float)((double)m * inv_temp + logf((float)s));
   } else {                                                      // unordered, all of them where they fit
     uint64_t* l = lists + (int64_t)blockIdx.x * len;
-    int all = (n[0] + n[1]) + (n[2] + n[3]);
-    if (all <= len) {
-      int before = 0;
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        for (int i = tid; i < n[g]; i += 256) l[before + i] = cand[g * TOP_WAVE + i];
-        before += n[g];
-      }
+    if (exact) {
+      for (int i = tid; i < kk; i += NT) l[i] = flat[i];
+    } else if (all <= len) {
+      for (int i = lane; i < n_own; i += 64) l[before_wave + i] = cand[w0 + i];
     } else {
-      rank_out<256, 4, TOP_WAVE>(cand, n, k, [&](int rank, uint64_t o) { l[rank] = o; });
+      rank_out<NT>(flat, all, k, [&](int rank, uint64_t o) { l[rank] = o; });
       all = kk;
     }
-    for (int i = all + tid; i < len; i += 256) l[i] = 0;
+    for (int i = all + tid; i < len; i += NT) l[i] = 0;
     if (tid == 0) parts[blockIdx.x] = {(double)m, s, exact || kk < k ? -INFINITY : thr};
   }
 }
@@ -390,30 +383,37 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
   for (int i = 0; i < 16; ++i)
     if (o[i] >= b0) cand[atomicAdd(&n_cand, 1)] = o[i];
   __syncthreads();
-  const int left[1] = {n_cand};
-  rank_out<NT, 1, 0>(cand, left, k, [&](int rank, uint64_t q) {
+  rank_out<NT>(cand, n_cand, k, [&](int rank, uint64_t q) {
     index[r * k + rank] = entry_id(q);
     values[r * k + rank] = D::put(key_value((uint32_t)(q >> 32)));
   });
-  if (threadIdx.x < 64) {
+  if (threadIdx.x >= NT - 64) {                                 // (the wavefront that ranks least)
     double m = -FLT_MAX, s = 0;
-    for (int i = threadIdx.x; i < n_chunk; i += 64) m = fmax(m, parts[r * n_chunk + i].m);
+    for (int i = threadIdx.x & 63; i < n_chunk; i += 64) m = fmax(m, parts[r * n_chunk + i].m);
     m = wave_max_d(m);
-    for (int i = threadIdx.x; i < n_chunk; i += 64) s += parts[r * n_chunk + i].s * exp((parts[r * n_chunk + i].m - m) * inv_temp);
+    for (int i = threadIdx.x & 63; i < n_chunk; i += 64) s += parts[r * n_chunk + i].s * exp((parts[r * n_chunk + i].m - m) * inv_temp);
     s = wave_sum_d(s);
-    if (threadIdx.x == 0) lse[r] = (float)(m * inv_temp + log(s));
+    if (threadIdx.x == NT - 1) lse[r] = (float)(m * inv_temp + log(s));
   }
 }
 
 // A chunk holds at most 16 vectors a thread, and not less than 16 k elements (or its list would be most of it).  Its list has room
 // for the candidates that a bound met by 5/4 k + 8 groups lets through, and at least k entries.
+// Few rows (no more than there are compute units) of up to 2^16 elements are taken by one workgroup of 1024 threads each, all in its
+// registers, without a join: 8 x 32000 fp32 k 16 9.0 us on the device against 10.1 in chunks, k 256 15.4 and 24.9, 256 x 50021 fp16 k 100
+// 13.5 and 18.4; but 400 x 32000 21.0 and 19.1, and 8 x 131072 bf16 k 64 16.9 and 14.1.
 struct TopPlan {
-  int n, chunk, len;
+  int n, chunk, len, threads;
 };
 static TopPlan top_plan(int rows, int V, int k, int dtype) {
   const int most = 256 * 16 * (16 / row_size(dtype));
   TopPlan t;
+  t.threads = 256;
   t.n = row_chunks(rows, V, most, 16 * k > 2048 ? 16 * k : 2048);
+  if (t.n > 1 && rows <= 256 && V <= 1 << 16) {
+    t.n = 1;
+    t.threads = 1024;
+  }
   if (t.n * k > TOP_MAX_LIST) t.n = row_chunks(512, V, most, V);
   t.chunk = (V + t.n - 1) / t.n;
   t.len = 2 * k + 32 < TOP_MAX_LIST / t.n ? 2 * k + 32 : TOP_MAX_LIST / t.n;
@@ -426,11 +426,11 @@ extern "C" int64_t nast_top_logits_workspace_bytes(int rows, int V, int k, int d
   return t.n > 1 ? (int64_t)rows * t.n * (t.len * (int64_t)sizeof(uint64_t) + (int64_t)sizeof(TopPart)) : 0;
 }
 
-template <class D, int NV>
+template <class D, int NT, int NV>
 static void top_launch(const void* x, nast_rows xr, void* values, int64_t* index, float* lse, uint64_t* lists, TopPart* parts, int rows,
                        int V, int k, TopPlan t, double temp, hipStream_t s) {
   using T = typename D::store;
-  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NV>), dim3(rows * t.n), dim3(256), 0, s, (const T*)x, xr, (T*)values, index, lse, lists, parts,
+  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NT, NV>), dim3(rows * t.n), dim3(NT), 0, s, (const T*)x, xr, (T*)values, index, lse, lists, parts,
                      V, k, t.len, t.chunk, t.n, 1.0 / temp, exp_scale(temp));
   if (t.n == 1) return;
   if (t.n * t.len <= 4096)
@@ -455,16 +455,21 @@ extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* val
   hipStream_t s = (hipStream_t)stream;
   uint64_t* lists = (uint64_t*)workspace;
   TopPart* parts = t.n > 1 ? (TopPart*)(lists + (int64_t)rows * t.n * t.len) : nullptr;
-  const int nv = (t.chunk / (16 / row_size(dtype)) + 255) / 256;      // vectors a thread
+  const int nv = (t.chunk / (16 / row_size(dtype)) + t.threads - 1) / t.threads;      // vectors a thread
   nast_prof_before(2, s);
-#define NAST_TOP(NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, t, temp, s)))
-  if (nv <= 2) NAST_TOP(2);
-  else if (nv <= 4) NAST_TOP(4);
-  else if (nv <= 6) NAST_TOP(6);
-  else if (nv <= 8) NAST_TOP(8);
-  else if (nv <= 10) NAST_TOP(10);
-  else if (nv <= 12) NAST_TOP(12);
-  else NAST_TOP(16);
+#define NAST_TOP(NT, NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NT, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, t, temp, s)))
+  if (t.threads == 1024) {
+    if (nv <= 2) NAST_TOP(1024, 2);
+    else if (nv <= 4) NAST_TOP(1024, 4);
+    else if (nv <= 8) NAST_TOP(1024, 8);
+    else top_launch<RowF32, 1024, 16>(x, xr, values, index, lse, lists, parts, rows, V, k, t, temp, s);   // (2^16 halves are 8)
+  } else if (nv <= 2) NAST_TOP(256, 2);
+  else if (nv <= 4) NAST_TOP(256, 4);
+  else if (nv <= 6) NAST_TOP(256, 6);
+  else if (nv <= 8) NAST_TOP(256, 8);
+  else if (nv <= 10) NAST_TOP(256, 10);
+  else if (nv <= 12) NAST_TOP(256, 12);
+  else NAST_TOP(256, 16);
 #undef NAST_TOP
   nast_prof_after(2, s, (double)row_size(dtype) * rows * (double)V);
   NAST_CHECK_LAUNCH("nast_top_logits");

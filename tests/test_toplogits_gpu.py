@@ -135,6 +135,27 @@ def test_top_logits_nans_in_one_chunk(ops, dtype):
         check_top(ops, x[:, :1500], k)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("R,V", [(257, 9001), (12, 9001), (12, 40001), (12, 65536), (12, 65537)])
+def test_top_logits_unusual_long_rows(ops, dtype, R, V):
+    """a row of each kind, in chunks and whole, at every alignment"""
+    for k in (1, 64, 256):
+        x = rows(R, V + 3, dtype, k)
+        x[0] = 0.37
+        x[1, ::3] = 9.0
+        x[2] = -INF
+        x[3, 5:-7] = -INF
+        x[4, 100:] = torch.finfo(dtype).min
+        x[5, ::7] = -float("nan")
+        x[6, ::2] = INF
+        x[7] = torch.where(torch.arange(V + 3, device="cuda") % 2 == 0, -0.0, 0.0).to(dtype)
+        x[8] = x[8].sort(descending=True).values
+        x[9] = x[9].sort().values
+        x[10, 2000:2400] += 30
+        for lead in (0, 1, 3):
+            check_top(ops, x[:, lead:lead + V], k)
+
+
 def test_top_logits_far_offsets(ops):
     """rows that lie beyond 2^31 elements of their tensor"""
     R, V = 20000, 120000
