@@ -480,6 +480,7 @@ extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* val
 // distillation
 // ---------------------------------------------------------------------------------------------
 #define DISTILL_MAX_K 256
+#define DISTILL_BWD_CHUNK 8192    // elements of a workgroup of the backward pass, up to twice as many
 #define DISTILL_NO_ID 0xffffffffu
 
 // teacher's list in its own type
@@ -497,6 +498,12 @@ struct DistillStats {
   double m_rest, coef, M, L, C, c;
 };
 
+// What a chunk leaves of its tokens; twice: some id of its part of the list stands in two slots.
+struct DistillPart {
+  double m, s;
+  int twice;
+};
+
 // What the list alone contributes to a row: with d_j = log p_j - (z_j - zm) / T up to the normalisers not known yet,
 //   S0 = sum e_j, S1 = sum e_j d_j, S2 = sum of exp((z - zm) / T) over the tokens named (each once), e_j = exp((t_j - C) / T - c0).
 // In double throughout: the loss is a small difference of terms near 1 (with one slot of p = 0.01 and q = 0.0075 it is 3e-4, while
@@ -506,11 +513,13 @@ struct SlotSums {
   bool any;
 };
 
-// By a workgroup of NT >= K threads, thread j = slot j; every thread gets the sums.  ids: LDS, holds the used slots' ids afterwards.
+// By a workgroup of NT >= K threads, thread j = slot j; every thread gets the sums.  ids: LDS, NT words at a multiple of 16 bytes, holds
+// the used slots' ids afterwards.  mark(id) is called for every used slot, twice() behind the barrier that follows: whether some id is
+// named by two of them.
 // Without TAIL no S2.
-template <class D, int NT, bool TAIL>
+template <class D, int NT, bool TAIL, class M, class W2>
 __device__ __forceinline__ SlotSums slot_sums(int64_t r, const typename D::store* p, const void* t, int t_dtype, const int64_t* idx, int K,
-                                              const float* lse_t, int V, double it, uint32_t* ids, double* red) {
+                                              const float* lse_t, int V, double it, uint32_t* ids, double* red, M&& mark, W2&& twice) {
   constexpr int W = NT / 64;
   const int j = threadIdx.x, w = threadIdx.x >> 6;
   uint32_t id = DISTILL_NO_ID;
@@ -521,9 +530,10 @@ __device__ __forceinline__ SlotSums slot_sums(int64_t r, const typename D::store
     if (slot_used(v, tj, V)) {
       id = (uint32_t)v;
       zj = D::get(p[v]);
+      mark((int)id);
     }
-    ids[j] = id;
   }
+  ids[j] = id;                               // (all NT: read in sixteens below)
   const bool used = id != DISTILL_NO_ID;
   float tm = wave_max(used ? tj : -FLT_MAX), zm = wave_max(used ? zj : -FLT_MAX);
   tm = fmaxf(tm, -FLT_MAX);
@@ -549,9 +559,23 @@ __device__ __forceinline__ SlotSums slot_sums(int64_t r, const typename D::store
     e = exp(a);
     if (e != 0) ed = e * (a - b);
     if (TAIL) {
-      bool first = true;                     // an id named twice is one token of the student's
-      for (int i = 0; i < j; ++i) first = first && ids[i] != id;
-      if (first) ez = exp(b);
+      int at = j;                            // an id named twice is one token of the student's: the first slot's
+      if (twice()) {
+#pragma unroll 1
+        for (int i = (K - 1) & ~15; i >= 0; i -= 16) {           // (sixteen at a time: one wait for LDS)
+          uint4 o[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) o[u] = *(const uint4*)(ids + i + 4 * u);
+#pragma unroll
+          for (int u = 3; u >= 0; --u) {
+            at = o[u].w == id ? i + 4 * u + 3 : at;
+            at = o[u].z == id ? i + 4 * u + 2 : at;
+            at = o[u].y == id ? i + 4 * u + 1 : at;
+            at = o[u].x == id ? i + 4 * u : at;
+          }
+        }
+      }
+      if (at == j) ez = exp(b);
     }
   }
   double any = __ballot(used) ? 1 : 0;
@@ -623,20 +647,21 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
                                                                    const void* __restrict__ t, int t_dtype,
                                                                    const int64_t* __restrict__ idx, int K,
                                                                    const float* __restrict__ lse_t, float* __restrict__ loss,
-                                                                   DistillStats* __restrict__ stats, MaxSumD* __restrict__ parts, int V,
+                                                                   DistillStats* __restrict__ stats, DistillPart* __restrict__ parts, int V,
                                                                    int chunk, int n_chunk, double it, float c) {
   constexpr int U = 4;
   extern __shared__ uint32_t bits[];                           // bit EPV + i: element body + i
   __shared__ double red[16];
-  __shared__ uint32_t ids[DISTILL_MAX_K];
+  __shared__ int twice;
+  __shared__ alignas(16) uint32_t ids[256];
   const unsigned block = gridDim.x - 1 - blockIdx.x;
   const int64_t r = block / n_chunk;
   const int lo = (int)(block % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
   MaxSum a{-FLT_MAX, 0.0};
   SlotSums q;
-  if (!SPLIT) q = slot_sums<D, 256, TAIL>(r, p, t, t_dtype, idx, K, lse_t, V, it, ids, red);
   if (!TAIL) {
+    if (!SPLIT) q = slot_sums<D, 256, TAIL>(r, p, t, t_dtype, idx, K, lse_t, V, it, ids, red, [](int) {}, [] { return false; });
     a = span_max_sum<D, 256>(p, lo, hi, c);
   } else {
     const RowSpan16<D> rs(p, lo, hi);
@@ -645,22 +670,22 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
     uint32_t* flags = bits + words;                            // byte (s / 1024) * 256 + s % 256, bit s / 256 % 4: vector s
     const int flag_words = (rs.n + 1023) / 1024 * 64;
     for (int w = threadIdx.x; w < words + flag_words; w += 256) bits[w] = 0;
-    uint32_t id = DISTILL_NO_ID;
-    if ((int)threadIdx.x < K) {
-      if (SPLIT) {
+    if (threadIdx.x == 0) twice = 0;
+    __syncthreads();
+    auto mark = [&](int id) {
+      const int bit = id - bit0, s = (id - rs.body) / D::EPV;
+      if (atomicOr(&bits[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1) twice = 1;
+      if (id >= rs.body && s < rs.n) atomicOr(&flags[(s >> 10) * 64 + ((s & 255) >> 2)], 1u << ((s & 3) * 8 + ((s >> 8) & 3)));
+    };
+    if (!SPLIT) {
+      q = slot_sums<D, 256, TAIL>(r, p, t, t_dtype, idx, K, lse_t, V, it, ids, red, mark, [&] { return twice != 0; });
+    } else {
+      if ((int)threadIdx.x < K) {
         const int64_t v = idx[r * K + threadIdx.x];
-        if (v >= lo && v < hi && slot_used(v, teacher_logit(t, t_dtype, r * K + threadIdx.x), V)) id = (uint32_t)v;
-      } else {
-        id = ids[threadIdx.x];
+        if (v >= lo && v < hi && slot_used(v, teacher_logit(t, t_dtype, r * K + threadIdx.x), V)) mark((int)v);
       }
+      __syncthreads();
     }
-    __syncthreads();
-    if (id != DISTILL_NO_ID) {
-      const int bit = (int)id - bit0, s = ((int)id - rs.body) / D::EPV;
-      atomicOr(&bits[bit >> 5], 1u << (bit & 31));
-      if ((int)id >= rs.body && s < rs.n) atomicOr(&flags[(s >> 10) * 64 + ((s & 255) >> 2)], 1u << ((s & 3) * 8 + ((s >> 8) & 3)));
-    }
-    __syncthreads();
     auto leave_out = [&](RowVec<D>& v, int slot) {
       const int at = (slot + 1) * D::EPV;
       const uint32_t named = bits[at >> 5] >> (at & 31);
@@ -692,7 +717,7 @@ __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typenam
   }
   const MaxSumD rest = block_max_sum<256>(a, c, red);
   if (threadIdx.x != 0) return;
-  if (SPLIT) parts[block] = rest;
+  if (SPLIT) parts[block] = {rest.m, rest.s, TAIL ? twice : 0};
   else distill_finish<TAIL>(r, rest, q, loss, stats, it);
 }
 
@@ -702,20 +727,24 @@ __global__ __launch_bounds__(NT) void nast_top_distill_join_kernel(const typenam
                                                                    const void* __restrict__ t, int t_dtype,
                                                                    const int64_t* __restrict__ idx, int K,
                                                                    const float* __restrict__ lse_t, float* __restrict__ loss,
-                                                                   DistillStats* __restrict__ stats, const MaxSumD* __restrict__ parts,
+                                                                   DistillStats* __restrict__ stats, const DistillPart* __restrict__ parts,
                                                                    int V, int n_chunk, double it) {
   __shared__ double red[NT / 16];
-  __shared__ uint32_t ids[NT];
+  __shared__ alignas(16) uint32_t ids[NT];
   const int64_t r = blockIdx.x;
   MaxSumD rest{-FLT_MAX, 0};
+  bool twice = false;
   for (int i = threadIdx.x & 63; i < n_chunk; i += 64) rest.m = fmax(rest.m, parts[r * n_chunk + i].m);
   rest.m = wave_max_d(rest.m);
   for (int i = threadIdx.x & 63; i < n_chunk; i += 64) {
-    const MaxSumD o = parts[r * n_chunk + i];
+    const DistillPart o = parts[r * n_chunk + i];
     rest.s += o.s * exp((o.m - rest.m) * it);
+    twice = twice || o.twice;
   }
   rest.s = wave_sum_d(rest.s);
-  const SlotSums q = slot_sums<D, NT, TAIL>(r, x + row_offset(r, xr), t, t_dtype, idx, K, lse_t, V, it, ids, red);
+  twice = __ballot(twice) != 0;
+  const SlotSums q = slot_sums<D, NT, TAIL>(r, x + row_offset(r, xr), t, t_dtype, idx, K, lse_t, V, it, ids, red,
+                                              [](int) {}, [&] { return twice; });
   if (threadIdx.x == 0) distill_finish<TAIL>(r, rest, q, loss, stats, it);
 }
 
@@ -731,8 +760,10 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
                                                                    typename D::store* __restrict__ gx, nast_rows gxr, int V, int chunk,
                                                                    int n_chunk, double it, float c) {
   constexpr int U = 4;
-  __shared__ uint32_t ids[DISTILL_MAX_K];
-  __shared__ float ts[DISTILL_MAX_K];
+  __shared__ uint32_t ids[256];              // the slots in this chunk, each wavefront's without gaps from 64 * its number
+  __shared__ double ps[256];
+  __shared__ uint32_t bits[DISTILL_BWD_CHUNK / 16];           // which elements are named: a chunk is shorter than two of these
+  __shared__ int cnt[4], twice;
   const int64_t r = blockIdx.x / n_chunk;
   const int lo = (int)(blockIdx.x % n_chunk) * chunk, hi = min(V, lo + chunk);
   const typename D::store* p = x + row_offset(r, xr);
@@ -740,17 +771,26 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
   const DistillStats st = stats[r];
   const double gr = (double)g[r] * it;
   uint32_t id = DISTILL_NO_ID;
-  float z = 0.f;
+  float z = 0.f, tv = 0.f;
   if ((int)threadIdx.x < K) {
     const int64_t v = idx[r * K + threadIdx.x];
-    const float tv = teacher_logit(t, t_dtype, r * K + threadIdx.x);
+    tv = teacher_logit(t, t_dtype, r * K + threadIdx.x);
     if (slot_used(v, tv, V) && v >= lo && v < hi) {
       id = (uint32_t)v;
       z = D::get(p[v]);
     }
-    ids[threadIdx.x] = id;
-    ts[threadIdx.x] = tv;
   }
+  for (int w = threadIdx.x; w < DISTILL_BWD_CHUNK / 16; w += 256) bits[w] = 0;
+  if (threadIdx.x == 0) twice = 0;
+  __syncthreads();
+  if (id != DISTILL_NO_ID && (atomicOr(&bits[((int)id - lo) >> 5], 1u << (((int)id - lo) & 31)) >> (((int)id - lo) & 31) & 1)) twice = 1;
+  const uint64_t named = __ballot(id != DISTILL_NO_ID);
+  const int own = (threadIdx.x & 192) + lanes_below(named);
+  if (id != DISTILL_NO_ID) {
+    ids[own] = id;
+    ps[own] = exp(((double)tv - st.C) * it - st.c);
+  }
+  if ((threadIdx.x & 63) == 0) cnt[threadIdx.x >> 6] = __popcll(named);
   // a factor of 0 (a row without a list, a row of no weight) writes zeros whatever the logits hold
   const float F = gr == 0 ? 0.f : (float)(gr * st.coef), m = (float)st.m_rest;
   const RowSpan16<D> rs(o, lo, hi);
@@ -773,12 +813,17 @@ __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* 
   if (e >= 0) o[e] = D::put(F == 0.f ? 0.f : exp_t(D::get(edge) - m, c) * F);
   __syncthreads();
   if (id == DISTILL_NO_ID) return;
-  double pj = 0;
+  double pj = ps[own];
   bool first = true;
-  for (int j = 0; j < K; ++j) {
-    if (ids[j] != id) continue;
-    first = first && j >= (int)threadIdx.x;
-    pj += exp(((double)ts[j] - st.C) * it - st.c);
+  if (twice) {                               // an id in two slots: the sum of both, by the first of them
+    pj = 0;
+    for (int w = 0; w < 4; ++w) {
+      for (int j = w * 64; j < w * 64 + cnt[w]; ++j) {
+        const bool same = ids[j] == id;
+        first = first && !(same && j < own);
+        pj += same ? ps[j] : 0.0;
+      }
+    }
   }
   if (first) o[id] = D::put(gr == 0 ? 0.f : (float)(gr * (exp(((double)z - st.M) * it - st.L) - pj)));
 }
@@ -805,12 +850,12 @@ static DistillPlan distill_plan(int rows, int V, int dtype) {
 extern "C" int64_t nast_top_distill_workspace_bytes(int rows, int V, int dtype) {
   if (rows < 1 || V < 1 || !row_dtype_ok(dtype)) return 0;
   const DistillPlan d = distill_plan(rows, V, dtype);
-  return d.n > 1 ? (int64_t)rows * d.n * (int64_t)sizeof(MaxSumD) : 0;
+  return d.n > 1 ? (int64_t)rows * d.n * (int64_t)sizeof(DistillPart) : 0;
 }
 
 template <class D, bool TAIL>
 static void distill_fwd(const void* x, nast_rows xr, const void* t, int t_dtype, const int64_t* idx, int K, const float* lse_t,
-                        float* loss, DistillStats* st, MaxSumD* parts, int rows, int V, DistillPlan d, double temp, hipStream_t s) {
+                        float* loss, DistillStats* st, DistillPart* parts, int rows, int V, DistillPlan d, double temp, hipStream_t s) {
   const typename D::store* xp = (const typename D::store*)x;
   const double it = 1.0 / temp;
   // bits of a chunk's elements, and of its vectors in fours of 256
@@ -842,7 +887,7 @@ extern "C" int nast_top_distill_fwd(const void* x, int dtype, nast_rows xr, cons
   NAST_REQUIRE(d.n == 1 || workspace, "nast_top_distill_fwd: NULL workspace");
   hipStream_t s = (hipStream_t)stream;
   DistillStats* st = (DistillStats*)stats;
-  MaxSumD* parts = (MaxSumD*)workspace;
+  DistillPart* parts = (DistillPart*)workspace;
   nast_prof_before(2, s);
   NAST_ROW_DTYPE(dtype, {
     if (lse_t) distill_fwd<D, true>(x, xr, t, t_dtype, idx, K, lse_t, loss, st, parts, rows, V, d, temp, s);
@@ -861,7 +906,7 @@ extern "C" int nast_top_distill_bwd(const float* g, const void* x, int dtype, na
   NAST_REQUIRE(g && x && t && idx && stats && gx, "nast_top_distill_bwd: NULL pointer");
   NAST_REQUIRE(x != gx, "nast_top_distill_bwd: in-place not supported");
   NAST_REQUIRE(row_aligned(x, dtype) && row_aligned(gx, dtype) && row_aligned(t, t_dtype), "nast_top_distill_bwd: misaligned pointer");
-  const int chunk = V < 8192 ? V : 8192, n = (V + chunk - 1) / chunk;
+  const int n = V < 2 * DISTILL_BWD_CHUNK ? 1 : V / DISTILL_BWD_CHUNK, chunk = (V + n - 1) / n;
   NAST_REQUIRE((int64_t)rows * n < (1 << 24), "nast_top_distill_bwd: too many rows (%d)", rows);
   nast_prof_before(2, (hipStream_t)stream);
   const bool around = (int64_t)rows * V * row_size(dtype) > (256 << 20);

@@ -248,6 +248,22 @@ def test_top_distill_slots(ops, dtype, tail):
 
 
 @pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("K", [40, 65, 256])
+@pytest.mark.parametrize("V", [9600, 16383, 16384, 40001])
+def test_top_distill_ids_in_many_slots(ops, V, K, tail):
+    """the same id in slots of one wavefront and of several, once, twice and everywhere, in rows beside others without"""
+    dtype = DTYPES[(V + K) % 3]
+    x = rows(5, V, dtype, K)
+    values, index, lse = teacher_of(x, K, 1.0, 2)
+    values = values - 2.0                                                # (some of them twice stay below a sum of one)
+    index[0, K // 2:2 * (K // 2)] = index[0, :K // 2]
+    index[1, 1::13] = index[1, 0]
+    index[2, -1] = index[2, 0]
+    index[3] = index[3, 0]
+    check_distill(ops, x, values, index, lse, 1.0, tail)
+
+
+@pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_top_distill_unusual_rows(ops, dtype, tail):
     V, K, temp = 1003, 6, 1.0
