@@ -12,7 +12,6 @@
 // ---------------------------------------------------------------------------------------------
 #define TOP_MAX_K 256
 #define TOP_MAX_V (1 << 20)
-#define TOP_WAVE 128              // candidates a wavefront keeps
 #define TOP_MAX_LIST 16384        // entries the join of a row's chunks takes
 
 // Elements are ordered by value, ties to the lower id: entry = key << 32 | ~id is one 64-bit number per element, no two alike, 0 is
@@ -21,14 +20,30 @@ __device__ __forceinline__ uint64_t top_entry(float f, int e) { return ((uint64_
 __device__ __forceinline__ int entry_id(uint64_t o) { return (int)~(uint32_t)o; }
 
 // n distinct entries in LDS: each goes to out(rank among all, entry) where the rank is below k.  A rank is a count of larger entries.
+// In workgroups of 1024, which few rows take, as many as 16 threads share an entry's comparisons (256 x 32000 fp32 k 256 17.4 -> 15.5 us);
+// with 256, which fill the card, one makes them all (4096 x 9600 fp16 k 200 60 us, shared 76).
 template <int NT, class F>
 __device__ __forceinline__ void rank_out(const uint64_t* cand, int n, int k, F&& out) {
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const uint64_t o = cand[i];
-    int rank = 0;
-#pragma unroll 4
-    for (int j = 0; j < n; ++j) rank += cand[j] > o ? 1 : 0;
-    if (rank < k) out(rank, o);
+  if constexpr (NT == 1024) {
+    int shift = 0;
+    while (shift < 4 && n << (shift + 1) <= NT) ++shift;
+    const int share = 1 << shift, part = threadIdx.x & (share - 1);
+    for (int i = threadIdx.x >> shift; i < n; i += NT >> shift) {
+      const uint64_t o = cand[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = part; j < n; j += share) rank += cand[j] > o ? 1 : 0;
+      for (int m = 1; m < share; m <<= 1) rank += __shfl_xor(rank, m, 64);
+      if (part == 0 && rank < k) out(rank, o);
+    }
+  } else {
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const uint64_t o = cand[i];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) rank += cand[j] > o ? 1 : 0;
+      if (rank < k) out(rank, o);
+    }
   }
 }
 
@@ -45,7 +60,7 @@ __device__ __forceinline__ int block_count(int n, int* cnt) {   // n <= 2^16 a t
 }
 
 // By one wavefront: bound[0] = a value that at least kk of the 64 * N group maxima reach (and, where one is found, not more than
-// 5/4 kk + 8), bound[1] = the largest.  Bisection on the upper half of the order key.
+// 9/8 kk + 8), bound[1] = the largest.  Bisection on the upper half of the order key.
 template <int N>
 __device__ __forceinline__ void group_bound(const float* gmax, int kk, float* bound) {
   const int lane = threadIdx.x & 63;
@@ -68,7 +83,7 @@ __device__ __forceinline__ void group_bound(const float* gmax, int kk, float* bo
     for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= mid));
     if (n >= kk) {
       b0 = mid;
-      if (n <= kk + kk / 4 + 8) break;
+      if (n <= kk + kk / 8 + 8) break;
     } else {
       b1 = mid;
     }
@@ -90,23 +105,23 @@ struct TopPart {
 // once.
 //
 // The k-th largest of the maxima of disjoint groups of elements is a lower bound of the k-th largest element.  Each thread keeps the
-// maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors) are the groups, and one
-// wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to LDS, each wavefront's to a place of
+// maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors, with up to two of them of
+// its elements) are the groups, and one wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to LDS, each wavefront's to a place of
 // its own, where its lanes look at their elements one by one; what reaches the bound (a little more than k elements where they lie at
-// random) is ranked by counting.  Where more than TOP_WAVE elements of a wavefront reach it (many equal values, e.g. a constant row), or
-// the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are taken in
-// the order of their ids.
+// random: 350 +- 19 of a large chunk for k = 256, a quarter of them to a wavefront) is ranked by counting.  Where more than `cap`
+// elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are
+// taken in the order of their ids.
 template <class D, int NT, int NV>
 __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
                                                              float* __restrict__ lse, uint64_t* __restrict__ lists,
-                                                             TopPart* __restrict__ parts, int V, int k, int len, int chunk, int n_chunk,
+                                                             TopPart* __restrict__ parts, int V, int k, int cap, int len, int chunk, int n_chunk,
                                                              double inv_temp, float c) {
-  constexpr int W = NT / 64, G = NT == 256 && NV >= 4 ? 4 : 1;
+  constexpr int W = NT / 64, G = NT == 256 ? 4 : 1;
   __shared__ float gmax[NT * G];
-  __shared__ uint64_t cand[W * TOP_WAVE];
-  __shared__ uint4 vec_data[W * TOP_WAVE];
-  __shared__ int vec_slot[W * TOP_WAVE];
+  extern __shared__ uint4 vec_data[];                           // for `cap` candidates a wavefront: vector, entry, slot
+  uint64_t* cand = (uint64_t*)(vec_data + W * cap);
+  int* vec_slot = (int*)(cand + W * cap);
   __shared__ double red[W];
   __shared__ int cnt[W];
   __shared__ float bound[2];
@@ -140,8 +155,12 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
   for (int i = 0; i < NV; ++i) {
     vm[i] = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < D::EPV; ++j) vm[i] = fmaxf(vm[i], v[i].get(j));
-    g[i % G] = fmaxf(g[i % G], vm[i]);
+    for (int j = 0; j < D::EPV; ++j) {
+      const float f = v[i].get(j);
+      vm[i] = fmaxf(vm[i], f);
+      if (NV < G) g[j % G] = fmaxf(g[j % G], f);
+    }
+    if (NV >= G) g[i % G] = fmaxf(g[i % G], vm[i]);
     __builtin_amdgcn_sched_barrier(0);
   }
   // from here the vectors are unpacked once more for the sum: the compiler must not keep what it has unpacked (half the kernel's
@@ -167,7 +186,7 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
   const float thr = bound[0], m = bound[1];
 
   // the wavefront's vectors that reach the bound, from registers into LDS
-  const int w0 = (tid >> 6) * TOP_WAVE;
+  const int w0 = (tid >> 6) * cap;
   int n_vec = 0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -175,7 +194,7 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
     const uint64_t all = __ballot(hit);
     if (all) {
       const int at = n_vec + lanes_below(all);
-      if (hit && at < TOP_WAVE) {
+      if (hit && at < cap) {
         vec_slot[w0 + at] = i * NT + tid;
         vec_data[w0 + at] = make_uint4(v[i].w[0], v[i].w[1], v[i].w[2], v[i].w[3]);
       }
@@ -205,9 +224,9 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
     n_own = __popcll(all);
   }
   const uint32_t* words = (const uint32_t*)(vec_data + w0);
-  for (int base = 0; base < min(n_vec, TOP_WAVE) * D::EPV; base += 64) {
+  for (int base = 0; base < min(n_vec, cap) * D::EPV; base += 64) {
     const int q = base + lane;
-    bool hit = q < min(n_vec, TOP_WAVE) * D::EPV;
+    bool hit = q < min(n_vec, cap) * D::EPV;
     float f = 0.f;
     if (hit) {
       f = D::unpack(words[q / RowVec<D>::PER], q % RowVec<D>::PER);
@@ -215,7 +234,7 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
     }
     const uint64_t all = __ballot(hit);
     const int at = n_own + lanes_below(all);
-    if (hit && at < TOP_WAVE) cand[w0 + at] = top_entry(f, rs.elem(vec_slot[w0 + q / D::EPV]) + q % D::EPV);
+    if (hit && at < cap) cand[w0 + at] = top_entry(f, rs.elem(vec_slot[w0 + q / D::EPV]) + q % D::EPV);
     n_own += __popcll(all);
   }
   if (lane == 0) {
@@ -234,7 +253,7 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
   }
 
   uint64_t* flat = (uint64_t*)vec_data;                         // the candidates without gaps
-  const bool exact = s != s || most > TOP_WAVE;
+  const bool exact = s != s || most > cap;
   if (exact) {                                 // (from memory again: a copy in registers would cost every row its place)
     constexpr int SHIFT = D::KEY_ZEROS;
     auto count = [&](uint64_t at_least) {                       // elements with key >> SHIFT at or above
@@ -379,9 +398,20 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
     }
   }
   __syncthreads();
+  int own = 0;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    if (o[i] >= b0) cand[atomicAdd(&n_cand, 1)] = o[i];
+    if (i * NT < n) own += __popcll(__ballot(o[i] >= b0));
+  int at = 0;                                                  // (each wavefront's place: in any order, they are ranked)
+  if ((threadIdx.x & 63) == 0 && own) at = atomicAdd(&n_cand, own);
+  at = __shfl(at, 0, 64);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (i * NT >= n) break;
+    const uint64_t all = __ballot(o[i] >= b0);
+    if (o[i] >= b0) cand[at + lanes_below(all)] = o[i];
+    at += __popcll(all);
+  }
   __syncthreads();
   rank_out<NT>(cand, n_cand, k, [&](int rank, uint64_t q) {
     index[r * k + rank] = entry_id(q);
@@ -398,12 +428,12 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
 }
 
 // A chunk holds at most 16 vectors a thread, and not less than 16 k elements (or its list would be most of it).  Its list has room
-// for the candidates that a bound met by 5/4 k + 8 groups lets through, and at least k entries.
+// for the candidates that a bound met by 9/8 k + 8 groups lets through, and at least k entries.
 // Few rows (no more than there are compute units) of up to 2^16 elements are taken by one workgroup of 1024 threads each, all in its
 // registers, without a join: 8 x 32000 fp32 k 16 9.0 us on the device against 10.1 in chunks, k 256 15.4 and 24.9, 256 x 50021 fp16 k 100
 // 13.5 and 18.4; but 400 x 32000 21.0 and 19.1, and 8 x 131072 bf16 k 64 16.9 and 14.1.
 struct TopPlan {
-  int n, chunk, len, threads;
+  int n, chunk, len, threads, cap;
 };
 static TopPlan top_plan(int rows, int V, int k, int dtype) {
   const int most = 256 * 16 * (16 / row_size(dtype));
@@ -416,6 +446,9 @@ static TopPlan top_plan(int rows, int V, int k, int dtype) {
   }
   if (t.n * k > TOP_MAX_LIST) t.n = row_chunks(512, V, most, V);
   t.chunk = (V + t.n - 1) / t.n;
+  // Candidates a wavefront has room for: more take the place of workgroups (4096 x 5003 fp32 k 256 62 us with 160, 80 with 256), but a row
+  // of two wavefronts' vectors has them all in those (4096 x 1000 fp16 k 256 98 and 76).
+  t.cap = t.threads == 1024 || k <= 128 ? 128 : t.chunk * row_size(dtype) <= 128 * 16 ? 256 : 160;
   t.len = 2 * k + 32 < TOP_MAX_LIST / t.n ? 2 * k + 32 : TOP_MAX_LIST / t.n;
   return t;
 }
@@ -430,8 +463,9 @@ template <class D, int NT, int NV>
 static void top_launch(const void* x, nast_rows xr, void* values, int64_t* index, float* lse, uint64_t* lists, TopPart* parts, int rows,
                        int V, int k, TopPlan t, double temp, hipStream_t s) {
   using T = typename D::store;
-  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NT, NV>), dim3(rows * t.n), dim3(NT), 0, s, (const T*)x, xr, (T*)values, index, lse, lists, parts,
-                     V, k, t.len, t.chunk, t.n, 1.0 / temp, exp_scale(temp));
+  hipLaunchKernelGGL((nast_top_chunk_kernel<D, NT, NV>), dim3(rows * t.n), dim3(NT),
+                     NT / 64 * t.cap * (sizeof(uint4) + sizeof(uint64_t) + sizeof(int)), s, (const T*)x, xr, (T*)values, index, lse, lists, parts, V,
+                     k, t.cap, t.len, t.chunk, t.n, 1.0 / temp, exp_scale(temp));
   if (t.n == 1) return;
   if (t.n * t.len <= 4096)
     hipLaunchKernelGGL((nast_top_join_kernel<D, 256>), dim3(rows), dim3(256), 0, s, lists, parts, (T*)values, index, lse, k, t.len, t.n,
