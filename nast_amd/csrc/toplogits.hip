@@ -111,6 +111,9 @@ struct TopPart {
 // random: 350 +- 19 of a large chunk for k = 256, a quarter of them to a wavefront) is ranked by counting.  Where more than `cap`
 // elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are
 // taken in the order of their ids.
+//
+// Bound by memory on long rows in numbers (16384 x 9600 fp32 105 us, 6.0 TB/s; 2048 x 131072 bf16 113 us with the join, 4.8 TB/s, where the
+// unpacking and exponentials of 16-bit elements take as long as their load), by latency below: 8 x 32000 fp32 9 us.
 template <class D, int NT, int NV>
 __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
@@ -347,7 +350,7 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
   }
 }
 
-// The lists of a row's chunks joined: 16 entries a thread, bisection until between k and 5 k / 4 + 32 of them are left, ranks by counting.
+// The lists of a row's chunks joined (one pass over a few KB, 8 to 13 us, latency): 16 entries a thread, bisection until between k and 5 k / 4 + 32 of them are left, ranks by counting.
 template <class D, int NT>
 __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __restrict__ lists, const TopPart* __restrict__ parts,
                                                            typename D::store* __restrict__ values, int64_t* __restrict__ index,
@@ -676,6 +679,7 @@ __device__ __forceinline__ void distill_finish(int64_t r, const MaxSumD& rest, c
 // and no difference.
 // Rows are taken from the last to the first: the backward pass, from the first to the last, then begins with what this pass has
 // left in the last-level cache (256 MB), and this pass with what the product that made the logits has left there.
+// Bound by memory: 16384 x 9600 fp32 with a tail 118 us (5.3 TB/s), 4096 x 131072 bf16 193 us (5.6 TB/s); 33 x 9600 fp32 6 us, latency.
 template <class D, bool SPLIT, bool TAIL>
 __global__ __launch_bounds__(256) void nast_top_distill_fwd_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                                    const void* __restrict__ t, int t_dtype,
@@ -784,8 +788,10 @@ __global__ __launch_bounds__(NT) void nast_top_distill_join_kernel(const typenam
 
 // One workgroup per chunk of a row: the rest's gradient everywhere, then, behind a barrier, the value of each named token over it.
 // AROUND: gradients of more than the last-level cache holds (256 MB) are stored around it, so that they do not drive out the logits the
-// forward pass has left there: 4096 x 131072 bf16 600 -> 572 us for both passes, 16384 x 9600 fp32 430 -> 390; a smaller one stays there
+// forward pass has left there: 4096 x 131072 bf16 577 -> 569 us for both passes, 16384 x 9600 fp32 388 -> 354; a smaller one stays there
 // for the product that reads it.
+// Bound by memory, one read and one write of the logits: 16384 x 9600 fp32 226 us (5.6 TB/s), 1021 x 50021 fp16 34 us (6.0 TB/s); 33 rows
+// of 9600 take 5 us, latency.  A chunk has 8192 elements or more, so that the list, read by each, is a small part of it.
 template <class D, bool AROUND>
 __global__ __launch_bounds__(256) void nast_top_distill_bwd_kernel(const float* __restrict__ g, const typename D::store* __restrict__ x,
                                                                    nast_rows xr, const void* __restrict__ t, int t_dtype,

@@ -332,7 +332,8 @@ __device__ __forceinline__ VerifyPair drafted_at(const VerifyArgs& A, int b, int
   return drafted<D>(A, b, i, row_pair(A, b * (A.N + 1) + i), A.draft ? row_pair(A, A.B * (A.N + 1) + b * A.N + i) : MaxSumD{0, 1});
 }
 
-// Between two rounds, one wavefront a sequence: whether a draft before place i0 is clearly refused.
+// Between two rounds, one wavefront a sequence: whether a draft before place i0 is clearly refused.  5 us, latency; without it each
+// workgroup of the round would find that out for itself.
 template <class D>
 __global__ __launch_bounds__(64) void nast_verify_ended_kernel(VerifyArgs A, int i0) {
   const int b = blockIdx.x, len = draft_length(A, b);
@@ -346,6 +347,8 @@ __global__ __launch_bounds__(64) void nast_verify_ended_kernel(VerifyArgs A, int
   if (threadIdx.x == 0) A.ended[b] = any != 0 || len < i0;
 }
 
+// One workgroup a chunk of a row: maximum and exponential sum.  Bound by memory: 268 MB of 256 sequences' first two places x 131072 bf16 in
+// 52 us (5.1 TB/s); sequences that have ended leave at once.
 template <class D>
 __global__ __launch_bounds__(256) void nast_verify_rows_kernel(VerifyArgs A, int i0, int n_target, int n_draft) {
   __shared__ double red[8];
@@ -409,7 +412,8 @@ __device__ void finish(const VerifyArgs& A, int b, int place, int len, const Ver
   if (threadIdx.x == 0) A.accepted[b] = place;
 }
 
-// One workgroup a sequence does everything.
+// One workgroup a sequence does everything behind the sums.  A chain of latencies: draft, its logits, place, p, q and E at that place,
+// scores, maxima; 12 us at 1 x 32000 bf16, 9 at 128 x 9600 fp32, of which 4 go before the place is known.
 template <class D, int NT>
 __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
   __shared__ double red[NT / 64];
@@ -420,8 +424,8 @@ __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
 }
 
 // One workgroup a chunk of a sequence.  Decisions that are too close are left to the join: the arithmetic in double would cost this
-// kernel, which has to fill the card, 22 registers and three of eight wavefronts.  (Where one of 256 x 131072 comes too close, about
-// one call in a hundred, the call takes 130 us more.)
+// kernel, which has to fill the card, 22 registers.  (Where one of 256 x 131072 comes too close, about one call in a hundred, the call
+// takes 130 us more.)  Bound by memory where there are rows enough: 256 x 131072 bf16, 268 MB of p, q and E in 48 us (5.6 TB/s).
 template <class D>
 __global__ __launch_bounds__(256) void nast_verify_chunk_kernel(VerifyArgs A) {
   __shared__ VerifyBest lds[4];
@@ -456,8 +460,8 @@ __global__ __launch_bounds__(1024) void nast_verify_join_kernel(VerifyArgs A) {
 
 // A further round costs two launches (10 us) and saves the rows of the sequences that have ended, half of them perhaps: it has to have
 // 128 MB of rows (20 us).  So many places at least has each, the first two or more, the next ones twice as many as the one before; where
-// less is left than that it is taken along.  256 x 8 drafts x 131072 bf16 in rounds of 2, 4, 3 places 199 us, at once 249; 512 x 32 x 9600
-// fp32 129 and 247; 64 x 8 x 131072 76 at once, 82 in the same three rounds.
+// less is left than that it is taken along.  256 x 8 drafts x 131072 bf16 in rounds of 2, 4, 3 places 196 us, at once 244; 512 x 32 x 9600
+// fp32 120 and 234; 64 x 8 x 131072 in rounds of 4 and 5 74, at once 80, in the three rounds 83.
 #define VERIFY_ROUND_BYTES (128 << 20)
 static int verify_round(const VerifyArgs& A, int dtype, int i0, int last) {
   const int64_t place = (int64_t)A.B * A.V * row_size(dtype) * (A.draft ? 2 : 1), least = (VERIFY_ROUND_BYTES + place - 1) / place;

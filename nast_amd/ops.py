@@ -1189,7 +1189,7 @@ def _positive(temperature):
 def top_logits(logits, k, temperature=1.0):
     """The k largest logits of every row of logits [..., V] and the row's log-sum-exp at `temperature`: TopLogits with values
     [..., k] (the logits' type, largest first, ties to the lower id, NaN above everything), index [..., k] int64, lse [...] fp32.
-    1 <= k <= min(256, V).  No gradient flows: this is the teacher's side."""
+    1 <= k <= min(256, V), V <= 2^20.  No gradient flows: this is the teacher's side."""
     if logits.requires_grad:
         logits = logits.detach()
     stream, dtype, temperature, k = _on_device(logits), _row_dtype(logits), _positive(temperature), int(k)
@@ -1283,7 +1283,8 @@ def top_distill(logits, top, temperature=1.0, tail=False):
     tail=False: c normalises the list itself.  tail=True: c = top.lse (taken at the same T), and what the list leaves out is one more
     class, with the teacher's 1 - sum p_j against the student's probability of every token outside the list.
     Slots whose id lies outside [0, V) (-1: the list ends early) or whose logit is -inf are unused; a row without a used slot has
-    loss 0 and gradient 0; an id in two slots counts in both.  Multiply by T * T for gradients of the usual scale."""
+    loss 0 and gradient 0; an id in two slots counts in both.  1 <= K <= 256, V < 2^24.  Multiply by T * T for gradients of the usual
+    scale."""
     return TopDistillFn.apply(logits, top, _positive(temperature), bool(tail))
 
 
@@ -1339,7 +1340,7 @@ def verify_draft(target, tokens, u, E, draft=None, lengths=None, temperature=1.0
 
     With p_i, q_i the softmax of the rows over `temperature`, draft i stands while u_i q_i(d_i) < p_i(d_i) (and q_i(d_i) > 0).  out
     holds the drafts that stand, then argmax (p_i - q_i)+ / E at the first that falls (p_N / E if none does), then -1.  A target row
-    without a distribution (a NaN, a +inf, nothing but -inf) lets nothing stand and gives -1."""
+    without a distribution (a NaN, a +inf, nothing but -inf) lets nothing stand and gives -1.  N <= 1024, V <= 2^20, B < 2^20."""
     stream, dtype, temperature = _on_device(target, tokens, u, E, draft, lengths), _row_dtype(target), _positive(temperature)
     if target.dim() != 3 or target.shape[1] < 1 or target.shape[2] < 1:
         raise _lib.NastHipError(f"target logits [B, N + 1, V] expected, got {tuple(target.shape)}")
