@@ -145,9 +145,12 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
 #pragma unroll
     for (int i = 0; i < NV; ++i) v[i] = vec_of<D>(-INFINITY);
   }
+  if (rs.n < NV * NT) {                                          // (a branch: whole chunks are spared the selects)
+    asm volatile("");
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    if ((i + 1) * NT > rs.n && i * NT + tid >= rs.n) v[i] = vec_of<D>(-INFINITY);
+    for (int i = 0; i < NV; ++i)
+      if ((i + 1) * NT > rs.n && i * NT + tid >= rs.n) v[i] = vec_of<D>(-INFINITY);
+  }
   const float ef = ee >= 0 ? D::get(edge) : -INFINITY;
 
   float vm[NV], g[G];
@@ -205,16 +208,29 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
     }
     __builtin_amdgcn_sched_barrier(0);
   }
-  float sum = exp_t(ef - m, c);
+  // 2^(x c - M) with one rounding and one instruction less than 2^((x - m) c); M is m c rounded, what that is off by is made good below.
+  // Beyond 2^24 that could be any power of two (and an infinite m has none): there the differences are taken, from memory once more.
+  const float M = m * c;
+  float sum = __builtin_amdgcn_exp2f(__builtin_fmaf(ef, c, -M));
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (i * NT < rs.n) {
       float t = 0.f;
 #pragma unroll
-      for (int j = 0; j < D::EPV; ++j) t += exp_t(v[i].get(j) - m, c);
+      for (int j = 0; j < D::EPV; ++j) t += __builtin_amdgcn_exp2f(__builtin_fmaf(v[i].get(j), c, -M));
       sum += t;
     }
     __builtin_amdgcn_sched_barrier(0);
+  }
+  if (!(fabsf(M) < 16777216.f)) {
+    sum = exp_t(ef - m, c);
+    for (int s = tid; s < rs.n; s += NT) {
+      const RowVec<D> w = rs.load(p, s);
+#pragma unroll
+      for (int j = 0; j < D::EPV; ++j) sum += exp_t(w.get(j) - m, c);
+    }
+  } else {
+    sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(m, c, -M));
   }
   const double ws = wave_sum_d((double)sum);
   // their elements, one to a lane

@@ -41,6 +41,9 @@ def check_top(ops, x, k, temp=1.0):
     want = flat.gather(1, index.cuda()).float()
     assert torch.equal(got.values.float().reshape(-1, k).nan_to_num(9e9), want.nan_to_num(9e9))
     lse_got = got.lse.cpu().double().reshape(-1)
+    over = lse.isfinite() & lse.float().isinf()           # beyond fp32's largest number, 3.4e38: its rounding is an infinity
+    assert torch.equal(lse_got[over], lse[over].float().double())
+    lse, lse_got = lse[~over], lse_got[~over]
     fine = lse.isfinite()
     assert torch.equal(lse_got[~fine].isnan(), lse[~fine].isnan() | (lse[~fine] == INF))
     assert ((lse_got - lse).abs()[fine] <= EPS + lse.abs()[fine] * 2.0 ** -24).all()
@@ -154,6 +157,21 @@ def test_top_logits_unusual_long_rows(ops, dtype, R, V):
         x[10, 2000:2400] += 30
         for lead in (0, 1, 3):
             check_top(ops, x[:, lead:lead + V], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("temp", [1.0, 1e-3, 1e-6, 1e20])
+def test_top_logits_magnitudes(ops, dtype, temp):
+    """rows whose largest logit over the temperature is tiny, around 2^24 and far beyond, of both signs"""
+    x = rows(12, 9001, dtype, 8)
+    for r, (scale, shift) in enumerate([(1e-6, 0), (1, 0), (1, 300), (1, -300), (1e3, 0), (100, 6e4), (100, -6e4), (1, 11629), (4, 23256)]):
+        x[r] = (x[r].float() * scale + shift).to(dtype)
+    if dtype != torch.float16:
+        x[9] = x[9] * 1e8
+        x[10] = x[10] * 1e37
+        x[11] = -x[11].abs() * 1e37
+    for n in (9001, 700):
+        check_top(ops, x[:, :n], 16, temp)
 
 
 def test_top_logits_far_offsets(ops):
