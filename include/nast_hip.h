@@ -180,7 +180,8 @@ int nast_first_eos_length_i64(const int64_t* tokens, int64_t* lengths, int B, in
 
 /* ------------------------------------------------------------------------------------------------
  * A teacher's top logits, distillation from them, verification of drafted tokens.  No counterpart in the reference.
- * Rows of logits in fp32, bf16 or fp16 (`dtype`); all arithmetic in fp32 or double.  `temp` > 0 divides the logits.
+ * Rows of logits in fp32, bf16 or fp16 (`dtype`); all arithmetic in fp32 or double.  `temp`, between
+ * 1e-30 and 1e30, divides the logits.
  * Sizes: lists of 1..256 slots; V <= 2^20, for distillation V < 2^24; fewer than 2^22 rows of several chunks, 2^24 of one.  Workspaces are
  * the caller's (sizes below; 256-byte aligned; 0 bytes: may be NULL), hold nothing between calls and must not be shared by calls that may
  * overlap.  Nothing is kept or allocated by the library, and all of it may be captured into a graph.

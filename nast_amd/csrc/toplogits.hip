@@ -106,14 +106,14 @@ struct TopPart {
 //
 // The k-th largest of the maxima of disjoint groups of elements is a lower bound of the k-th largest element.  Each thread keeps the
 // maximum of each of its vectors; their maxima over a thread (or, for k > 64, over a quarter of its vectors, with up to two of them of
-// its elements) are the groups, and one wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to LDS, each wavefront's to a place of
-// its own, where its lanes look at their elements one by one; what reaches the bound (a little more than k elements where they lie at
-// random: 350 +- 19 of a large chunk for k = 256, a quarter of them to a wavefront) is ranked by counting.  Where more than `cap`
-// elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are
-// taken in the order of their ids.
+// its elements) are the groups, and one wavefront finds a bound among them (group_bound).  Vectors whose maximum reaches the bound go to
+// LDS, each wavefront's to a place of its own, where its lanes look at their elements one by one; what reaches the bound (a little more
+// than k elements where they lie at random: 350 +- 19 of a large chunk for k = 256, a quarter of them to a wavefront) is ranked by
+// counting.  Where more than `cap` elements of a wavefront reach it (many equal values, e.g. a constant row), or the row holds a NaN, the
+// k-th key is found exactly instead, by bisection with a count over the chunk, and equal elements are taken in the order of their ids.
 //
-// Bound by memory on long rows in numbers (16384 x 9600 fp32 105 us, 6.0 TB/s; 2048 x 131072 bf16 113 us with the join, 4.8 TB/s, where the
-// unpacking and exponentials of 16-bit elements take as long as their load), by latency below: 8 x 32000 fp32 9 us.
+// Bound by memory on long rows in numbers (16384 x 9600 fp32 105 us, 6.0 TB/s; 2048 x 131072 bf16 113 us with the join, 4.8 TB/s, where
+// the unpacking and exponentials of 16-bit elements take as long as their load), by latency below: 8 x 32000 fp32 9 us.
 template <class D, int NT, int NV>
 __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D::store* __restrict__ x, nast_rows xr,
                                                              typename D::store* __restrict__ values, int64_t* __restrict__ index,
@@ -366,7 +366,8 @@ __global__ __launch_bounds__(NT, 4) void nast_top_chunk_kernel(const typename D:
   }
 }
 
-// The lists of a row's chunks joined (one pass over a few KB, 8 to 13 us, latency): 16 entries a thread, bisection until between k and 5 k / 4 + 32 of them are left, ranks by counting.
+// The lists of a row's chunks joined (a few KB, 8 to 13 us, latency): 16 entries a thread, bisection until between k and 5 k / 4 + 32 of
+// them are left, ranks by counting.
 template <class D, int NT>
 __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __restrict__ lists, const TopPart* __restrict__ parts,
                                                            typename D::store* __restrict__ values, int64_t* __restrict__ index,
@@ -426,10 +427,11 @@ __global__ __launch_bounds__(NT) void nast_top_join_kernel(const uint64_t* __res
   at = __shfl(at, 0, 64);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    if (i * NT >= n) break;
-    const uint64_t all = __ballot(o[i] >= b0);
-    if (o[i] >= b0) cand[at + lanes_below(all)] = o[i];
-    at += __popcll(all);
+    if (i * NT < n) {
+      const uint64_t all = __ballot(o[i] >= b0);
+      if (o[i] >= b0) cand[at + lanes_below(all)] = o[i];
+      at += __popcll(all);
+    }
   }
   __syncthreads();
   rank_out<NT>(cand, n_cand, k, [&](int rank, uint64_t q) {
@@ -499,7 +501,7 @@ extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* val
   NAST_REQUIRE(row_dtype_ok(dtype), "nast_top_logits: unknown dtype %d", dtype);
   NAST_REQUIRE(rows >= 0 && V >= 1 && V <= TOP_MAX_V, "nast_top_logits: bad sizes rows=%d V=%d", rows, V);
   NAST_REQUIRE(k >= 1 && k <= TOP_MAX_K && k <= V, "nast_top_logits: k=%d must lie in [1, %d] and not exceed V=%d", k, TOP_MAX_K, V);
-  NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_top_logits: temperature must be > 0 and finite");
+  NAST_REQUIRE(temp > 1e-30 && temp < 1e30, "nast_top_logits: temperature must lie between 1e-30 and 1e30");
   if (rows == 0) return NAST_OK;
   const TopPlan t = top_plan(rows, V, k, dtype);
   NAST_REQUIRE((int64_t)rows * t.n < (t.n == 1 ? 1 << 24 : 1 << 22), "nast_top_logits: too many rows (%d)", rows);
@@ -888,7 +890,7 @@ static int distill_check(const char* name, int dtype, int t_dtype, int K, int ro
   NAST_REQUIRE(row_dtype_ok(dtype) && row_dtype_ok(t_dtype), "%s: unknown dtype", name);
   NAST_REQUIRE(rows >= 0 && V >= 1 && V < (1 << 24), "%s: bad sizes rows=%d V=%d", name, rows, V);
   NAST_REQUIRE(K >= 1 && K <= DISTILL_MAX_K, "%s: a list has 1 to %d slots, not %d", name, DISTILL_MAX_K, K);
-  NAST_REQUIRE(temp > 0 && temp < 1e30, "%s: temperature must be > 0 and finite", name);
+  NAST_REQUIRE(temp > 1e-30 && temp < 1e30, "%s: temperature must lie between 1e-30 and 1e30", name);
   return NAST_OK;
 }
 // One workgroup reads a whole row where there are rows enough to fill the card (512: two workgroups a compute unit); a chunk has at

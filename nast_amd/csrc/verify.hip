@@ -503,7 +503,7 @@ extern "C" int nast_verify_draft(const void* target, int64_t target_bs, int64_t 
   NAST_REQUIRE(row_dtype_ok(dtype), "nast_verify_draft: unknown dtype %d", dtype);
   NAST_REQUIRE(B >= 0 && B < (1 << 20) && N >= 0 && N <= VERIFY_MAX_DRAFTS && V >= 1 && V <= VERIFY_MAX_V,
                "nast_verify_draft: bad sizes B=%d N=%d V=%d", B, N, V);
-  NAST_REQUIRE(temp > 0 && temp < 1e30, "nast_verify_draft: temperature must be > 0 and finite");
+  NAST_REQUIRE(temp > 1e-30 && temp < 1e30, "nast_verify_draft: temperature must lie between 1e-30 and 1e30");
   if (B == 0) return NAST_OK;
   NAST_REQUIRE(target && E && out && accepted && workspace && (N == 0 || (tokens && u)),
                "nast_verify_draft: NULL pointer");

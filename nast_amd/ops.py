@@ -1181,8 +1181,8 @@ def _workspace(like, name, *sizes):
 
 def _positive(temperature):
     t = float(temperature)
-    if not 0 < t < 1e30:
-        raise _lib.NastHipError(f"temperature must be > 0 and finite, got {t}")
+    if not 1e-30 < t < 1e30:
+        raise _lib.NastHipError(f"temperature must lie between 1e-30 and 1e30, got {t}")
     return t
 
 

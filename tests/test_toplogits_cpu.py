@@ -33,7 +33,7 @@ def test_cpu_tensors_are_refused():
         ops.verify_draft(torch.zeros(2, 2, 8), torch.zeros(2, 1, dtype=torch.int64), torch.zeros(2, 1), torch.ones(2, 8))
 
 
-@pytest.mark.parametrize("t", [0.0, -1.0, math.inf, math.nan])
+@pytest.mark.parametrize("t", [0.0, -1.0, 1e-40, math.inf, math.nan])
 def test_temperature_is_refused(t):
     with pytest.raises(_lib.NastHipError, match="temperature"):
         ops.top_distill(torch.zeros(2, 8), None, t)
