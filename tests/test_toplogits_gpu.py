@@ -626,6 +626,18 @@ def test_verify_draft_strides(ops, dtype):
     assert out.shape == (0, 6) and accepted.shape == (0,)
 
 
+def test_verify_draft_far_offsets(ops):
+    """rows that lie beyond 2^31 elements of their tensor"""
+    V = 120000
+    base = torch.zeros(4500, 4, V, dtype=torch.bfloat16, device="cuda")
+    target, tokens, u, E, draft = drafts(4, 3, V, torch.bfloat16, 9)
+    base[::1499], base[1::1499, :3] = target, draft
+    far_target, far_draft = base[::1499], base[1::1499, :3]
+    assert far_target.stride(0) * 3 > 1 << 31
+    check_verify(ops, far_target, tokens, u, E, far_draft)
+    check_verify(ops, far_target, tokens, u * 0, E, far_draft)
+
+
 def test_verify_draft_distribution(ops):
     """the tokens that come out follow the target, wherever the drafts came from: frequencies within 5 standard deviations"""
     import nast_amd.utils as U
