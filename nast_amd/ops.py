@@ -1186,6 +1186,11 @@ def _positive(temperature):
     return t
 
 
+def _per_row(lead, dev):
+    # (sizes one by one: torch takes 0.8 us longer to read them from a torch.Size)
+    return torch.empty(*lead, device=dev, dtype=F32) if lead else torch.empty((), device=dev, dtype=F32)
+
+
 def top_logits(logits, k, temperature=1.0):
     """The k largest logits of every row of logits [..., V] and the row's log-sum-exp at `temperature`: TopLogits with values
     [..., k] (the logits' type, largest first, ties to the lower id, NaN above everything), index [..., k] int64, lse [...] fp32.
@@ -1200,7 +1205,7 @@ def top_logits(logits, k, temperature=1.0):
     lead = logits.shape[:-1]
     values = torch.empty(*lead, k, device=x.device, dtype=x.dtype)
     index = torch.empty(*lead, k, device=x.device, dtype=torch.int64)
-    lse = torch.empty(lead, device=x.device, dtype=F32)
+    lse = _per_row(lead, x.device)
     ws = _workspace(x, "nast_top_logits_workspace_bytes", rows, V, k, dtype)
     call("nast_top_logits", _p(x), dtype, r, _p(values), _p(index), _p(lse), rows, V, k, temperature, _p(ws), stream)
     return TopLogits(values, index, lse, temperature)
@@ -1229,7 +1234,7 @@ def _distill_fwd(x, r, rows, lead, dtype, teacher, temperature, stream):
     """-> loss [lead] fp32, stats [rows, 6] double"""
     values, index, lse = teacher
     V, dev = x.shape[-1], x.device
-    loss = torch.empty(lead, device=dev, dtype=F32)
+    loss = _per_row(lead, dev)
     stats = torch.empty(rows, 6, device=dev, dtype=torch.float64)
     ws = _workspace(x, "nast_top_distill_workspace_bytes", rows, V, dtype)
     call("nast_top_distill_fwd", _p(x), dtype, r, _p(values), _ROW_DTYPES[values.dtype], _p(index), values.shape[-1], _p(lse), _p(loss),
