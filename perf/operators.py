@@ -160,7 +160,7 @@ def _plain_distill(x, values, index, lse_t, temp, tail, g):
     # in 64 bits: the loss is a small difference of sums over the whole vocabulary
     vocab = x.shape[1]
     z = x.detach().double() / temp
-    used = (index >= 0) & (index < vocab) & (values != -math.inf)
+    used = (index >= 0) & (index < vocab)
     some = used.any(1)
     at = index.clamp(0, vocab - 1)
     t = torch.where(used, values.double() / temp, -math.inf)
@@ -180,8 +180,7 @@ def _plain_distill(x, values, index, lse_t, temp, tail, g):
         inside = torch.zeros_like(z).scatter_add_(1, at, used.double()) > 0
         p_rest = (1.0 - p.sum(1, keepdim=True)).clamp(min=0.0)
         q_rest = torch.where(inside, 0.0, e).sum(1, keepdim=True) / s
-        both = (p_rest > 0) & (q_rest > 0)
-        loss = loss + torch.where(both, p_rest * (p_rest.log() - q_rest.log()), 0.0).squeeze(1)
+        loss = loss + torch.where(p_rest > 0, p_rest * (p_rest.log() - q_rest.log()), 0.0).squeeze(1)
         ratio = torch.where(q_rest > 0, p_rest / q_rest, 0.0)
         dz = torch.where(inside, dz, dz * (1.0 - ratio))
     dz = dz.scatter_add_(1, at, torch.where(used, -p, 0.0)) * (g / temp).unsqueeze(1)
@@ -287,7 +286,7 @@ def _exact_distill(state):
     for r in range(0, case["rows"], step):
         index, t = state["index"][r:r + step], state["values"][r:r + step].double() / case["temp"]
         z = (x[r:r + step].double() / case["temp"]).requires_grad_()
-        good = (index >= 0) & (index < case["vocab"]) & (t > -math.inf)
+        good = (index >= 0) & (index < case["vocab"])
         logq = torch.log_softmax(z, 1)
         t = torch.where(good, t, torch.full_like(t, -math.inf))
         empty = ~good.any(1)
@@ -302,8 +301,7 @@ def _exact_distill(state):
             row = torch.arange(index.shape[0], device=x.device).unsqueeze(1).expand_as(index)
             mask[row[good], index[good]] = True
             log_rest = torch.logsumexp(logq.masked_fill(mask, -math.inf), 1)
-            some = (rest > 0) & (log_rest > -math.inf)
-            loss = loss + torch.where(some, torch.xlogy(rest, rest) - rest * log_rest, 0.0)
+            loss = loss + torch.where(rest > 0, torch.xlogy(rest, rest) - rest * log_rest, 0.0)
         loss = torch.where(empty, 0.0, loss)
         # d loss / d logits = d loss / d z / temp
         (grad,) = torch.autograd.grad((loss * state["grad_loss"][r:r + step].double()).sum(), z)
