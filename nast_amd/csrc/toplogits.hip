@@ -3,8 +3,10 @@
 //   top:      the k largest logits of a row with their ids, and lse = log sum_v exp(x_v / T)
 //   distill:  p_j = exp(t_j / T - c) over the used slots j of the teacher's list, q = softmax(z / T),
 //             loss = sum_j p_j (log p_j - log q_{id_j})  [+ p_r (log p_r - log q_r)]
-//             dz_v = g / T * (q_v - [rest] p_r q_v / q_r - sum_{j: id_j = v} p_j)
-//             p_r = 1 - sum p_j and q_r = sum of q over the tokens no used slot names: the rest bucket (only with the teacher's lse)
+//             dz_v = g / T * (w q_v - [rest] p_r q_v / q_r - sum_{j: id_j = v} p_j)
+//             p_r = max(0, 1 - sum p_j) and q_r = sum of q over the tokens no used slot names: the rest bucket (only with the teacher's
+//             lse, and only where q_r > 0);  w = sum p_j + p_r of the bucket kept: every term holds the normaliser of log q once.  w is 1
+//             but where the list is more than one (its logits rounded, its lse not; an id in two slots) or the bucket has nothing
 #include "rowvec.h"
 
 // ---------------------------------------------------------------------------------------------
@@ -548,7 +550,8 @@ __device__ __forceinline__ float teacher_logit(const void* t, int dtype, int64_t
 __device__ __forceinline__ bool slot_used(int64_t id, float t, int V) { return id >= 0 && id < V && t != -INFINITY; }
 
 // What the backward pass needs of a row: the rest's maximum and the factor of its exponentials, and the normalisers of
-// log q_v = (z_v - M) / T - L and log p_j = (t_j - C) / T - c (in two parts: next to a logit of -3e38 a logarithm of a sum would be lost).
+// log (w q_v) = (z_v - M) / T - L and log p_j = (t_j - C) / T - c (in two parts: next to a logit of -3e38 a logarithm of a sum would be
+// lost).
 struct DistillStats {
   double m_rest, coef, M, L, C, c;
 };
@@ -677,9 +680,11 @@ __device__ __forceinline__ void distill_finish(int64_t r, const MaxSumD& rest, c
     const double log_qr = below + log(rest.s) - o.L;
     const double pr = rest.s == 0 ? 0.0 : fmax(1.0 - q.S0, 0.0);   // (no bucket where the student has no token left for it)
     if (pr > 0) l += pr * (log(pr) - log_qr);
-    // q_v - p_r q_v / q_r = exp((z_v - m_r) / T) / s_r * (q_r - p_r): no quotient of small numbers; 0 for a row without a rest, NaN
+    const double w = q.S0 + pr;
+    // w q_v - p_r q_v / q_r = exp((z_v - m_r) / T) / s_r * (w q_r - p_r): no quotient of small numbers; 0 for a row without a rest, NaN
     // for a row of nothing but -inf
-    o.coef = rest.s == 0 ? (o.L > -INFINITY ? 0.0 : NAN) : (exp(log_qr) - pr) / rest.s;
+    o.coef = rest.s == 0 ? (o.L > -INFINITY ? 0.0 : NAN) : (w * exp(log_qr) - pr) / rest.s;
+    o.L -= log(w);                           // (+inf where w is 0: such a row's gradient is 0)
   } else {
     o.M = rest.m;
     o.L = log(rest.s);

@@ -35,16 +35,18 @@ def distill(logits, values, index, lse, temp, tail, g):
         logq = z - z.exp().sum().log()
         q = logq.exp()
         loss = torch.where(p != 0, p * ((tj - c) - logq[at]), 0.0).sum()
-        dz, size = q.clone(), q.clone()
         rest = torch.ones(V, dtype=torch.bool)
         rest[at] = False
+        mass, bucket = p.sum(), 0.0                           # of all the terms of the loss; what the rest bucket takes from q
         if tail:
             pr, log_qr = max(0.0, 1.0 - p.sum().item()), torch.logsumexp(logq[rest], 0) if rest.any() else torch.tensor(-math.inf).double()
             if pr > 0 and log_qr > -math.inf:
                 loss = loss + pr * (math.log(pr) - log_qr)
+                mass = mass + pr
                 bucket = pr * (logq[rest] - log_qr).exp()
-                dz[rest] -= bucket
-                size[rest] += bucket
+        dz, size = mass * q, mass * q                         # log q_v = z_v - logsumexp(z), in every term: q_v times their mass
+        dz[rest] -= bucket
+        size[rest] += bucket
         for j, v in enumerate(at.tolist()):
             dz[v] -= p[j]
             size[v] += p[j]
