@@ -103,8 +103,15 @@ __device__ __forceinline__ float exp_t(float t, float c) { return __builtin_amdg
 // Sum of exponentials relative to a maximum.  The maximum starts at the lowest finite value, so that no -inf is subtracted from
 // -inf: a row of -inf ends with s = 0 (log-sum-exp -inf), a row of the type's lowest value counts as any other row.  A NaN or
 // +inf among the elements leaves s = NaN.  Vectors are summed in fp32 (at most 32 terms), everything from there in double.
-// What s is off by, relative: 4e-6.  An exponential 2^-a has 3 roundings of its argument, 1.24e-7 * a, and the instruction's 1.2e-7;
-// weighted by the exponentials themselves a is log2(V) <= 20 on average at most (entropy); 12 roundings of a sum add 7e-7.
+// What a row's s is off by, relative.  An element's term is a product of powers 2^-a: its own, and one for each time the sum it is in was
+// brought to a larger maximum: at most R times in its thread (once a batch of for_slots and once for the edge), then over the wavefront, the
+// workgroup and the row's chunks.  A power has 3 roundings of its argument (difference, product, c), 1.24e-7 * a, and the instruction's
+// 1.2e-7 (one unit; 8.5e-8 measured over [-1, 0]).  The a's of an element add up to log2 of the largest term over its own; weighted by
+// the terms that is 15.2 on average at most for V = 2^20 and 18.9 for 2^24 (one element with 0.09 or 0.07 of the sum, the others alike).
+// 12 roundings of a sum add 7e-7:  1.24e-7 * 15.2 + 1.2e-7 * (R + 4) + 7e-7.
+//   chunks of 2^15 elements (verification): 8 batches whole, or 7, 4 vectors and an edge: R = 12, 4.5e-6, below ROW_SUM_REL
+//   chunks of 2^15 vectors (distillation): 32 batches, or 31, 4 vectors and an edge: R = 36, 7.9e-6 for V = 2^24
+#define ROW_SUM_REL 5e-6
 struct MaxSum {
   float m;
   double s;

@@ -11,9 +11,13 @@
 
 #define VERIFY_MAX_V (1 << 20)
 #define VERIFY_MAX_DRAFTS 1024
-// What the fp32 probabilities of the draw are off by, relative: the row's sum 4e-6 (see MaxSum), an exponent of -a before and of up to
-// a + 20 after the sum's logarithm is added ln 2 * 2^-24 * (4 a + 40), the instruction 1.2e-7.
-#define VERIFY_REL 6e-6f
+// Sums are off by ROW_SUM_REL each (see MaxSum): a draft's two probabilities are told apart where they differ by more than both, and by
+// what doubles add.
+#define VERIFY_CLOSE 1.1e-5
+// What the fp32 probabilities of the draw are off by, relative: the row's sum 5e-6, an exponent of -a before and of up to a + 20 after the
+// sum's logarithm is added ln 2 * 2^-24 * (4 a + 40) = 1.65e-7 a + 1.65e-6, the instruction 1.2e-7; a score's difference, sum with its bound,
+// reciprocal and product 3e-7.  7.1e-6 in all, and 1.65e-7 a.
+#define VERIFY_REL 7.5e-6f
 #define VERIFY_REL_EXP 2e-7f
 
 struct VerifyArgs {
@@ -103,7 +107,7 @@ __device__ __forceinline__ VerifyPair drafted(const VerifyArgs& A, int b, int i,
 }
 __device__ __forceinline__ bool stands(const VerifyPair& r, float u) { return r.q > 0 && (double)u * r.q < r.p; }
 __device__ __forceinline__ bool too_close(const VerifyPair& r, float u) {
-  return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= 1e-5 * r.p;   // (two sums)
+  return r.p > 0 && r.q > 0 && fabs((double)u * r.q - r.p) <= VERIFY_CLOSE * r.p;
 }
 // the same decision with sums in double, by the whole workgroup
 template <class D, int NT, int U>
@@ -310,18 +314,27 @@ __device__ int race_exact(const VerifyArgs& A, int b, const VerifyDraw& w, float
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ MaxSumD row_pair(const VerifyArgs& A, int row) {
   const MaxSumD* q = A.parts + (int64_t)row * A.n_chunk;
-  MaxSumD t = q[0];
-  for (int i = 1; i < A.n_chunk; i += 4) {                     // four loads in flight
-    MaxSumD o[4];
+  if (A.n_chunk == 1) return proper(q[0]);
+  // the maximum first: each chunk's sum is then brought to it by one exponential, whatever order the maxima come in
+  MaxSumD o[4], t;                                             // four loads in flight
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = q[min(i + j, A.n_chunk - 1)];
+  for (int j = 0; j < 4; ++j) o[j] = q[min(j, A.n_chunk - 1)];
+  t.m = fmax(fmax(o[0].m, o[1].m), fmax(o[2].m, o[3].m));
+  for (int i = 4; i < A.n_chunk; i += 4) {
+    double m[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i + j >= A.n_chunk) break;
-      const double m = fmax(t.m, o[j].m);
-      t.s = t.s * (double)exp_t((float)(t.m - m), A.c) + o[j].s * (double)exp_t((float)(o[j].m - m), A.c);
-      t.m = m;
+    for (int j = 0; j < 4; ++j) m[j] = q[min(i + j, A.n_chunk - 1)].m;
+    t.m = fmax(t.m, fmax(fmax(m[0], m[1]), fmax(m[2], m[3])));
+  }
+  t.s = 0;
+  for (int i = 0; i < A.n_chunk; i += 4) {
+    if (i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = q[min(i + j, A.n_chunk - 1)];
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j < A.n_chunk) t.s += o[j].s * (double)exp_t((float)(o[j].m - t.m), A.c);
   }
   return proper(t);
 }
