@@ -1230,6 +1230,15 @@ def _teacher_list(lead, top, temperature, tail):
     return _c(values), _c(index), _c(lse)
 
 
+def pick_top(top, lead, index, temperature=1.0, tail=False):
+    """The rows `index` [R] int64 of a TopLogits of rows [*lead], as a TopLogits of [R] rows.  It is checked against `lead` before: picked
+    from another layout, rows of the wrong places would fit.  The log-sum-exp is kept only where the tail needs it."""
+    values, ids, lse = _teacher_list(lead, top, _positive(temperature), tail)
+    _on_device(index, values, ids, lse)
+    pick = lambda t: t.flatten(0, len(lead) - 1).index_select(0, index)
+    return TopLogits(pick(values), pick(ids), None if lse is None else pick(lse), top.temperature)
+
+
 def _distill_fwd(x, r, rows, lead, dtype, teacher, temperature, stream):
     """-> loss [lead] fp32, stats [rows, 6] double"""
     values, index, lse = teacher

@@ -295,10 +295,7 @@ class Decoder(nn.Module):
             nll = self.generator.nll(z, temperature, tok).view(-1)[:sub.total]
             return torch.zeros(B * (n - 1), device=x.device, dtype=nll.dtype).index_copy(0, sub.idx, nll).view(B, n - 1)
         if teacher_top is not None:                             # padded positions come back as 0
-            if tuple(teacher_top.index.shape[:-1]) != (B, n - 1):
-                raise ops._lib.NastHipError(f"teacher_top: lists [{B}, {n - 1}, K] expected, got {tuple(teacher_top.index.shape)}")
-            pick = lambda t: None if t is None else t.flatten(0, 1).index_select(0, sub.idx_p)
-            top = ops.TopLogits(pick(teacher_top.values), pick(teacher_top.index), pick(teacher_top.lse), teacher_top.temperature)
+            top = ops.pick_top(teacher_top, (B, n - 1), sub.idx_p, temperature, teacher_tail)
             loss = self.generator.distill(z, temperature, top, teacher_tail)[:sub.total]
             return torch.zeros(B * (n - 1), device=x.device, dtype=loss.dtype).index_copy(0, sub.idx, loss).view(B, n - 1)
         if packed_out:                                          # log-probs of the real positions only: [sub.rows, V]
