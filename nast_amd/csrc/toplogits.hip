@@ -514,6 +514,10 @@ extern "C" int nast_top_logits(const void* x, int dtype, nast_rows xr, void* val
   TopPart* parts = t.n > 1 ? (TopPart*)(lists + (int64_t)rows * t.n * t.len) : nullptr;
   const int nv = (t.chunk / (16 / row_size(dtype)) + t.threads - 1) / t.threads;      // vectors a thread
   nast_prof_before(2, s);
+  // Vectors a thread: the next even number up to 12, else 16; a wider kernel's spare vectors cost registers and selects.  Two or four too
+  // many: 28086 x 5600 fp32, k 32, 121 us with 6, 140 with 8; 16384 x 9600 110 with 10, 128 with 12; 13355 x 11777 113 with 12, 121
+  // with 16; halves and k 200 alike.  14 is left out: 11234 x 14000 fp32 112.4 us with 16, 110.6 with 14; 28000 bf16 124.9 and 120.8.
+  // Workgroups of 1024, for calls of 9 to 20 us: powers of two; 12 for 16 and 6 for 8 would save 0.2 to 1 us (8 x 40001 fp32 11.4, 10.4).
 #define NAST_TOP(NT, NV) NAST_ROW_DTYPE(dtype, (top_launch<D, NT, NV>(x, xr, values, index, lse, lists, parts, rows, V, k, t, temp, s)))
   if (t.threads == 1024) {
     if (nv <= 2) NAST_TOP(1024, 2);

@@ -426,7 +426,7 @@ __device__ void finish(const VerifyArgs& A, int b, int place, int len, const Ver
 }
 
 // One workgroup a sequence does everything behind the sums.  A chain of latencies: draft, its logits, place, p, q and E at that place,
-// scores, maxima; 12 us at 1 x 32000 bf16, 9 at 128 x 9600 fp32, of which 4 go before the place is known.
+// scores, maxima; 13 us at 1 x 32000 bf16, 10 at 128 x 9600 fp32, of which 4 go before the place is known.
 template <class D, int NT>
 __global__ __launch_bounds__(NT) void nast_verify_draw_kernel(VerifyArgs A) {
   __shared__ double red[NT / 64];
